@@ -624,6 +624,42 @@ def sparse_softmax_cross_entropy_with_logits(labels=None, logits=None, name=None
         labels=dense, logits=logits, name=name or "sparse_softmax_cross_entropy_with_logits")
 
 
+def layer_norm(x, scale=None, offset=None, epsilon: float = 1e-5, name=None) -> Tensor:
+    """``(x - mean) / sqrt(variance + epsilon) * scale + offset`` with the mean and variance of
+    every row of ``x``'s last dimension. ``scale`` / ``offset``: vectors of that dimension
+    (``None``: 1 / 0) in ``x``'s dtype or fp32; fp32, bf16 and fp16 inputs. Differentiable in all
+    three."""
+    x = convert_to_tensor(x)
+    if x.dtype.name not in ("float32", "bfloat16", "float16"):
+        raise TypeError("layer_norm: fp32, bf16 or fp16 input, got %s" % x.dtype.name)
+    if x.shape is None or len(x.shape) == 0 or not x.shape[-1]:
+        raise ValueError("layer_norm needs a static last dimension of at least one element, got "
+                         "shape %s" % (x.shape,))
+    if not epsilon >= 0.0:
+        raise ValueError("layer_norm: epsilon must not be negative, got %r" % (epsilon,))
+    inputs, present = [x], []
+    for param, what in ((scale, "scale"), (offset, "offset")):
+        present.append(param is not None)
+        if param is None:
+            continue
+        param = convert_to_tensor(param)
+        if param.shape is not None and tuple(param.shape) != (x.shape[-1],):
+            raise ValueError("layer_norm: %s has shape %s for rows of %d"
+                             % (what, param.shape, x.shape[-1]))
+        if param.dtype != x.dtype and param.dtype != dtypes.float32:
+            raise TypeError("layer_norm: %s is %s for %s input" % (what, param.dtype.name,
+                                                                    x.dtype.name))
+        inputs.append(param)
+    if len(inputs) == 3 and inputs[1].dtype != inputs[2].dtype:
+        raise TypeError("layer_norm: scale is %s, offset %s" % (inputs[1].dtype.name,
+                                                                inputs[2].dtype.name))
+    stats = (dtypes.float32, tuple(x.shape[:-1]))
+    return _g(inputs).create_op(
+        "LayerNorm", inputs, [(x.dtype, x.shape), stats, stats], name=name or "LayerNorm",
+        attrs={"epsilon": float(epsilon), "has_scale": present[0],
+               "has_offset": present[1]}).outputs[0]
+
+
 def mean_squared_error(labels, predictions, name=None) -> Tensor:
     """``mean((predictions - labels) ** 2)`` over all elements as one fused op (forward: partial
     sums + fold; backward: one element-wise launch) when both have the same static shape; the
@@ -946,6 +982,20 @@ def _softmax_grad(op, g):
 def _log_softmax_grad(op, g):
     y = op.outputs[0]
     return (_op1("LogSoftmaxGrad", [y, g], y.dtype, y.shape, name="LogSoftmaxGrad"),)
+
+
+@gradient("LayerNorm")
+def _layer_norm_grad(op, g, g_mean=None, g_rstd=None):
+    """The statistics are outputs for the backward pass only: nothing differentiates them."""
+    x = op.inputs[0]
+    has_scale, has_offset = op.attrs["has_scale"], op.attrs["has_offset"]
+    params = op.inputs[1:]
+    node = op.graph.create_op(
+        "LayerNormGrad", [g, x, op.outputs[1], op.outputs[2]] + ([params[0]] if has_scale else []),
+        [(x.dtype, x.shape)] + [(p.dtype, p.shape) for p in params], name="LayerNormGrad",
+        attrs={"has_scale": has_scale, "has_offset": has_offset,
+               "param_dtype": params[0].dtype if params else dtypes.float32})
+    return tuple(node.outputs)
 
 
 @gradient("SoftmaxCrossEntropyWithLogits")

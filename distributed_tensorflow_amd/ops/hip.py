@@ -184,6 +184,8 @@ def _declare(L: ctypes.CDLL) -> None:
         "dtf_one_hot_f32": [P, I, P, LG, LG, F, F, P],
         "dtf_broadcast_mid_f32": [P, P, LG, LG, LG, F, P],
         "dtf_log_softmax_grad_f32": [P, P, P, LG, LG, P],
+        "dtf_layer_norm": [P, LG, I, P, P, I, P, P, P, LG, LG, F, P],
+        "dtf_layer_norm_grad": [P, LG, P, LG, I, P, P, P, I, P, P, P, P, LG, LG, P],
         "dtf_absmax_scale": [P, I, LG, F, P, P, P],
         "dtf_cast_to_fp8_dev_scale": [P, I, P, LG, P, P],
         "dtf_truncated_normal_f32": [P, LG, U, U, F, F, P],
@@ -202,6 +204,8 @@ def _declare(L: ctypes.CDLL) -> None:
     L.dtf_absmax_workspace.restype = LG
     L.dtf_mx_scale_bytes.argtypes = [LG, LG]
     L.dtf_mx_scale_bytes.restype = LG
+    L.dtf_layer_norm_grad_workspace.argtypes = [LG, LG, I]
+    L.dtf_layer_norm_grad_workspace.restype = LG
 
 
 # ---------------------------------------------------------------------------------------
@@ -1957,6 +1961,131 @@ def log_softmax_grad(y: torch.Tensor, dy: torch.Tensor) -> torch.Tensor:
                                           y2.shape[0], y2.shape[1], _stream()),
            "log_softmax_grad")
     return dx.view(y.shape)
+
+
+_NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _on_device(t: torch.Tensor):
+    """Context in which launches go to ``t``'s device (nothing to do when it is the current one)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _norm_rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """``t`` as a matrix of its last dimension's rows: contiguous rows at any pitch are taken as
+    they lie, anything else is copied."""
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise HipKernelError("%s: expected a GPU tensor" % what)
+    if t.dtype not in _NORM_TYPES:
+        raise HipKernelError("%s: expected fp32, bf16 or fp16, got %s" % (what, t.dtype))
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise HipKernelError("%s: needs a last dimension of at least one element, got shape %s"
+                             % (what, tuple(t.shape)))
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
+
+
+def _norm_param(p: Optional[torch.Tensor], x: torch.Tensor, what: str) -> Optional[torch.Tensor]:
+    if p is None:
+        return None
+    if not isinstance(p, torch.Tensor) or p.device != x.device:
+        raise HipKernelError("%s: expected a tensor on the input's GPU" % what)
+    if p.dtype != x.dtype and p.dtype != torch.float32:
+        raise HipKernelError("%s: expected fp32 or the input's %s, got %s"
+                             % (what, x.dtype, p.dtype))
+    if p.numel() != x.shape[-1]:
+        raise HipKernelError("%s: %d elements for rows of %d" % (what, p.numel(), x.shape[-1]))
+    return p if p.is_contiguous() else p.contiguous()
+
+
+def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None,
+               beta: Optional[torch.Tensor] = None, epsilon: float = 1e-5,
+               want_stats: bool = False):
+    """``(x - mean) / sqrt(var + epsilon) * gamma + beta`` over the last dimension of ``x`` (fp32,
+    bf16 or fp16; rows at any pitch), rounded once to ``x``'s type. ``gamma`` / ``beta``: fp32 or
+    ``x``'s type (both the same), ``None`` for 1 / 0. ``want_stats``: returns ``(y, mean, rstd)``
+    with the fp32 statistics ``layer_norm_grad`` takes, of shape ``x.shape[:-1]``."""
+    x2 = _norm_rows(x, "layer_norm x")
+    gamma = _norm_param(gamma, x, "layer_norm gamma")
+    beta = _norm_param(beta, x, "layer_norm beta")
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise HipKernelError("layer_norm: gamma and beta differ in dtype")
+    if not epsilon >= 0.0:
+        raise HipKernelError("layer_norm: epsilon must not be negative, got %r" % (epsilon,))
+    p = gamma if gamma is not None else beta
+    rows, cols = x2.shape
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if want_stats else None
+    if rows:
+        base = stats.data_ptr() if want_stats else 0
+        with _on_device(x):
+            _check(lib().dtf_layer_norm(
+                x2.data_ptr(), x2.stride(0), _NORM_TYPES[x.dtype], _ptr(gamma), _ptr(beta),
+                _NORM_TYPES[p.dtype if p is not None else torch.float32], y.data_ptr(),
+                base or None, base + 4 * rows if base else None, rows, cols, float(epsilon),
+                _stream()), "layer_norm")
+    if not want_stats:
+        return y
+    mean, rstd = stats.unbind(0)
+    if x.dim() != 2:
+        mean, rstd = mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
+    return y, mean, rstd
+
+
+def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                    gamma: Optional[torch.Tensor] = None, want_gamma: bool = True,
+                    want_beta: bool = True, param_dtype: Optional[torch.dtype] = None,
+                    dgamma_out: Optional[torch.Tensor] = None,
+                    dbeta_out: Optional[torch.Tensor] = None):
+    """Gradients of ``layer_norm``: ``(dx, dgamma, dbeta)`` from ``dy``, the input ``x`` and the
+    ``mean`` / ``rstd`` its forward returned; a parameter gradient that is not wanted is ``None``.
+    ``dx`` has ``x``'s type, ``dgamma`` / ``dbeta`` (column sums taken in fp32, in a fixed order)
+    ``gamma``'s -- ``param_dtype`` when there is no ``gamma`` (default fp32). ``dgamma_out`` /
+    ``dbeta_out``: contiguous fp32 buffers for fp32 parameter gradients."""
+    x2, dy2 = _norm_rows(x, "layer_norm_grad x"), _norm_rows(dy, "layer_norm_grad dy")
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise HipKernelError("layer_norm_grad: dy and x differ in shape, dtype or device")
+    gamma = _norm_param(gamma, x, "layer_norm_grad gamma")
+    rows, cols = x2.shape
+    for t, what in ((mean, "mean"), (rstd, "rstd")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != x.device \
+                or t.numel() != rows:
+            raise HipKernelError("layer_norm_grad: %s must hold one fp32 per row" % what)
+    mean = mean if mean.is_contiguous() else mean.contiguous()
+    rstd = rstd if rstd.is_contiguous() else rstd.contiguous()
+    p_dtype = gamma.dtype if gamma is not None else (param_dtype or torch.float32)
+    if p_dtype != x.dtype and p_dtype != torch.float32:
+        raise HipKernelError("layer_norm_grad: parameter gradients are fp32 or the input's %s"
+                             % x.dtype)
+    kind = _NORM_TYPES[x.dtype]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    sums = []
+    for want, out in ((want_gamma, dgamma_out), (want_beta, dbeta_out)):
+        if not want:
+            sums.append(None)
+        elif out is None:
+            sums.append(torch.empty((cols,), dtype=p_dtype, device=x.device))
+        elif p_dtype != torch.float32 or out.device != x.device:
+            raise HipKernelError("layer_norm_grad: bad out tensor")
+        else:
+            sums.append(_out_vec(out, cols, x.device, "layer_norm_grad"))
+    dgamma, dbeta = sums
+    L = lib()
+    ws = None
+    if want_gamma or want_beta:
+        ws = torch.empty((L.dtf_layer_norm_grad_workspace(rows, cols, kind),),
+                         dtype=torch.float32, device=x.device)
+    with _on_device(x):
+        _check(L.dtf_layer_norm_grad(
+            dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), kind, mean.data_ptr(),
+            rstd.data_ptr(), _ptr(gamma), _NORM_TYPES[p_dtype], dx.data_ptr(), _ptr(ws),
+            _ptr(dgamma), _ptr(dbeta), rows, cols, _stream()), "layer_norm_grad")
+    return dx, dgamma, dbeta
 
 
 def absmax_scale(x: torch.Tensor, target: float = FP8_MAX) -> torch.Tensor:

@@ -465,6 +465,26 @@ def _argmax_accuracy(op, inputs, ctx):
     return [hip.argmax_accuracy(y, labels)]
 
 
+@hip_kernel("LayerNorm")
+def _layer_norm(op, inputs, ctx):
+    scale = inputs[1] if op.attrs["has_scale"] else None
+    offset = inputs[-1] if op.attrs["has_offset"] else None
+    return list(hip.layer_norm(inputs[0], scale, offset, op.attrs["epsilon"], want_stats=True))
+
+
+@hip_kernel("LayerNormGrad")
+def _layer_norm_grad(op, inputs, ctx):
+    dy, x, mean, rstd = inputs[:4]
+    has_scale, has_offset = op.attrs["has_scale"], op.attrs["has_offset"]
+    n = x.shape[-1]
+    dt = op.attrs["param_dtype"].torch
+    dx, dscale, doffset = hip.layer_norm_grad(
+        dy, x, mean, rstd, inputs[4] if has_scale else None, has_scale, has_offset, dt,
+        dgamma_out=_hint(ctx, 1, (n,)) if has_scale and dt == _f32 else None,
+        dbeta_out=_hint(ctx, 1 + has_scale, (n,)) if has_offset and dt == _f32 else None)
+    return [dx] + [t for t in (dscale, doffset) if t is not None]
+
+
 # -- shape plumbing / bookkeeping with real data movement ------------------------------------
 @hip_kernel("Transpose")
 def _transpose(op, inputs, ctx):

@@ -553,6 +553,38 @@ def _sxent(op, inputs, ctx):
     return [loss, backprop]
 
 
+@ref_kernel("LayerNorm")
+def _layer_norm(op, inputs, ctx):
+    """(x[, scale][, offset]) -> (y, mean, rstd): rows of the last dimension, fp32 arithmetic."""
+    x = inputs[0].float()
+    params = [p.float() for p in inputs[1:]]
+    mean = x.mean(dim=-1, keepdim=True)
+    d = x - mean
+    rstd = 1.0 / torch.sqrt((d * d).mean(dim=-1, keepdim=True) + op.attrs["epsilon"])
+    y = d * rstd
+    if op.attrs["has_scale"]:
+        y = y * params[0]
+    if op.attrs["has_offset"]:
+        y = y + params[-1]
+    return [y.to(inputs[0].dtype), mean.squeeze(-1), rstd.squeeze(-1)]
+
+
+@ref_kernel("LayerNormGrad")
+def _layer_norm_grad(op, inputs, ctx):
+    """(dy, x, mean, rstd[, scale]) -> (dx[, dscale][, doffset])."""
+    dy, x = inputs[0].float(), inputs[1].float()
+    rstd = inputs[3].unsqueeze(-1)
+    h = (x - inputs[2].unsqueeze(-1)) * rstd
+    g = dy * inputs[4].float() if op.attrs["has_scale"] else dy
+    dx = rstd * (g - g.mean(dim=-1, keepdim=True) - h * (g * h).mean(dim=-1, keepdim=True))
+    outs, dt, n = [dx.to(inputs[1].dtype)], op.attrs["param_dtype"].torch, x.shape[-1]
+    if op.attrs["has_scale"]:
+        outs.append((dy * h).reshape(-1, n).sum(dim=0).to(dt))
+    if op.attrs["has_offset"]:
+        outs.append(dy.reshape(-1, n).sum(dim=0).to(dt))
+    return outs
+
+
 @ref_kernel("RowScale")
 def _row_scale(op, inputs, ctx):
     x, s = inputs
