@@ -184,6 +184,8 @@ def _declare(L: ctypes.CDLL) -> None:
         "dtf_one_hot_f32": [P, I, P, LG, LG, F, F, P],
         "dtf_broadcast_mid_f32": [P, P, LG, LG, LG, F, P],
         "dtf_log_softmax_grad_f32": [P, P, P, LG, LG, P],
+        "dtf_newton_schulz": [I, P, P, P, P, I, I, P, F, P, LG, P],
+        "dtf_multi_muon_f32": [I, P, P, P, P, P, P, I, P, F, F, P, F, I, F, P, LG, P],
         "dtf_layer_norm": [P, LG, I, P, P, I, P, P, P, LG, LG, F, P],
         "dtf_layer_norm_grad": [P, LG, P, LG, I, P, P, P, I, P, P, P, P, LG, LG, P],
         "dtf_absmax_scale": [P, I, LG, F, P, P, P],
@@ -204,6 +206,8 @@ def _declare(L: ctypes.CDLL) -> None:
     L.dtf_absmax_workspace.restype = LG
     L.dtf_mx_scale_bytes.argtypes = [LG, LG]
     L.dtf_mx_scale_bytes.restype = LG
+    L.dtf_newton_schulz_workspace.argtypes = [I, P, P]
+    L.dtf_newton_schulz_workspace.restype = LG
     L.dtf_layer_norm_grad_workspace.argtypes = [LG, LG, I]
     L.dtf_layer_norm_grad_workspace.restype = LG
 
@@ -1289,6 +1293,152 @@ def multi_optim(rule: str, params: Sequence[torch.Tensor], grads: Sequence[torch
                                          len(hyper), pw[0], pw[1],
                                          None if lr is None else lr.data_ptr(), _stream()),
                "multi_optim")
+
+
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_NS_GROUP = 16          # matrices of one launch sequence
+
+
+def _ns_coefficients(coefficients, steps: int, what: str):
+    """ctypes array of (a, b, c) per step from one triple or a triple for every step."""
+    if not isinstance(steps, int) or not 1 <= steps <= 32:
+        raise HipKernelError("%s: steps must be 1..32, got %r" % (what, steps))
+    rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else coefficients
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise HipKernelError("%s: coefficients are one (a, b, c) or one for each of the %d steps"
+                             % (what, steps))
+    return (ctypes.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
+
+
+def _ns_workspace(shapes, device, what: str):
+    n = len(shapes)
+    rows = (ctypes.c_int * n)(*[s[0] for s in shapes])
+    cols = (ctypes.c_int * n)(*[s[1] for s in shapes])
+    size = lib().dtf_newton_schulz_workspace(n, rows, cols)
+    if size <= 0:
+        raise HipKernelError("%s: matrices of up to 2^22 rows and columns, got %s"
+                             % (what, list(shapes)))
+    ws = torch.empty((size,), dtype=torch.uint8, device=device)
+    base = (ws.data_ptr() + 255) // 256 * 256
+    return rows, cols, ws, base, ws.data_ptr() + size - base
+
+
+def _ns_check(code: int, what: str) -> None:
+    if code == -2:
+        raise HipKernelError("%s: these coefficients let a singular value in [0, 1] grow beyond "
+                             "the range of the 16-bit images (3.5)" % what)
+    _check(code, what)
+
+
+def newton_schulz(g, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
+                  epsilon: float = 1e-7):
+    """Orthogonalised ``g`` -- a matrix, a stack of matrices (rank 3) or a list of matrices of any
+    shapes, fp32, bf16 or fp16: ``X = g / (|g|_F + epsilon)``, then ``steps`` times ``A = X X^T;
+    X = a X + (b A + c A A) X`` on the orientation with fewer rows. Every singular value is moved
+    towards one and the singular vectors are kept. ``coefficients``: one (a, b, c), or one per
+    step; a polynomial under which a singular value in [0, 1] grows beyond 3.5 is refused. The
+    products keep 22 bits of every operand and accumulate in fp32; the result is rounded once, to
+    ``g``'s dtype. Up to 16 matrices share one sequence of launches."""
+    what = "newton_schulz"
+    if isinstance(g, torch.Tensor):
+        mats = [g] if g.dim() == 2 else list(g) if g.dim() == 3 else None
+    else:
+        mats = list(g)
+    if mats is None or any(not isinstance(t, torch.Tensor) or t.dim() != 2 for t in mats):
+        raise HipKernelError("newton_schulz: a matrix, a stack of matrices or a list of matrices")
+    if isinstance(g, torch.Tensor) and g.device.type != "cuda":
+        raise HipKernelError("newton_schulz: expected a GPU tensor")
+    if not epsilon >= 0.0:
+        raise HipKernelError("newton_schulz: epsilon must not be negative, got %r" % (epsilon,))
+    coef = _ns_coefficients(coefficients, steps, what)
+    for t in mats:
+        if t.dtype not in _NORM_TYPES or t.device != mats[0].device or t.dtype != mats[0].dtype:
+            raise HipKernelError("newton_schulz: matrices of one dtype (fp32, bf16 or fp16) on "
+                                 "one GPU")
+        if t.device.type != "cuda":
+            raise HipKernelError("newton_schulz: expected a GPU tensor")
+    if isinstance(g, torch.Tensor):
+        result = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        outs = [result] if g.dim() == 2 else list(result)
+    else:
+        result = outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in mats]
+    work = [(t if t.is_contiguous() else t.contiguous(), o) for t, o in zip(mats, outs)
+            if t.numel()]
+    for start in range(0, len(work), _NS_GROUP):
+        part = work[start:start + _NS_GROUP]
+        n, t0 = len(part), part[0][0]
+        with _on_device(t0):
+            rows, cols, ws, base, size = _ns_workspace([t.shape for t, _ in part], t0.device, what)
+            g_arr = (ctypes.c_void_p * n)(*[t.data_ptr() for t, _ in part])
+            o_arr = (ctypes.c_void_p * n)(*[o.data_ptr() for _, o in part])
+            _ns_check(lib().dtf_newton_schulz(n, g_arr, o_arr, rows, cols, _NORM_TYPES[t0.dtype],
+                                              steps, coef, float(epsilon), base, size, _stream()),
+                      what)
+    return result
+
+
+def muon_scale(rows: int, cols: int) -> float:
+    """Learning-rate factor of a [inputs, outputs] matrix under the Muon rule."""
+    return max(1.0, cols / rows) ** 0.5 if rows else 1.0
+
+
+def multi_muon(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
+               moments: Sequence[torch.Tensor], lr, momentum: float = 0.95,
+               nesterov: bool = True, weight_decay: float = 0.0,
+               scales: Optional[Sequence[float]] = None, steps: int = 5,
+               coefficients=NEWTON_SCHULZ_COEFFICIENTS, epsilon: float = 1e-7) -> None:
+    """In-place Muon update of fp32 matrices (or stacks of them, rank 3): ``v = momentum v + g``;
+    ``u = g + momentum v`` (``nesterov``; else ``v``); ``w = (1 - lr weight_decay) w - lr scale
+    newton_schulz(u)``. ``scales``: one factor per parameter, default ``sqrt(max(1, outputs /
+    inputs))`` of its [inputs, outputs]. ``lr``: a number, or an fp32 device scalar read when the
+    kernels run. Up to 16 matrices of any shapes share one sequence of launches."""
+    what = "multi_muon"
+    if len(params) != len(grads) or len(params) != len(moments) or \
+            (scales is not None and len(scales) != len(params)):
+        raise HipKernelError("multi_muon: argument lists differ in length")
+    lr_dev = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device.type != "cuda":
+            raise HipKernelError("multi_muon: lr must be a number or an fp32 GPU scalar")
+        lr, lr_dev = 0.0, lr
+    if not epsilon >= 0.0:
+        raise HipKernelError("multi_muon: epsilon must not be negative, got %r" % (epsilon,))
+    coef = _ns_coefficients(coefficients, steps, what)
+    work = []
+    spans = []
+    for i, (p, g, m) in enumerate(zip(params, grads, moments)):
+        for t in (p, g, m):
+            if t.dtype != torch.float32 or t.device.type != "cuda" or t.device != params[0].device \
+                    or t.shape != p.shape or p.dim() not in (2, 3):
+                raise HipKernelError("multi_muon: params, grads and moments must be matching fp32 "
+                                     "GPU matrices or stacks of matrices")
+        if not p.is_contiguous() or not m.is_contiguous():
+            raise HipKernelError("multi_muon: params and moments must be contiguous")
+        if p.numel() == 0:
+            continue
+        g = g if g.is_contiguous() else g.contiguous()
+        spans += [(t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in (p, m)]
+        scale = float(scales[i]) if scales is not None else muon_scale(*p.shape[-2:])
+        work += [(a, b, c, scale) for a, b, c in
+                 (zip(p, g, m) if p.dim() == 3 else ((p, g, m),))]
+    spans.sort()
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise HipKernelError("multi_muon: params and moments overlap in memory")
+    if lr_dev is not None and work and lr_dev.device != work[0][0].device:
+        raise HipKernelError("multi_muon: lr is on another device")
+    c = ctypes
+    for start in range(0, len(work), _NS_GROUP):
+        part = work[start:start + _NS_GROUP]
+        n, w0 = len(part), part[0][0]
+        with _on_device(w0):
+            rows, cols, ws, base, size = _ns_workspace([w.shape for w, _, _, _ in part],
+                                                       w0.device, what)
+            arrays = [(c.c_void_p * n)(*[t[k].data_ptr() for t in part]) for k in range(3)]
+            s_arr = (c.c_float * n)(*[t[3] for t in part])
+            _ns_check(lib().dtf_multi_muon_f32(
+                n, arrays[0], arrays[1], arrays[2], s_arr, rows, cols, steps, coef,
+                float(epsilon), float(lr), _ptr(lr_dev), float(momentum), int(bool(nesterov)),
+                float(weight_decay), base, size, _stream()), what)
 
 
 def affine_scalars(scalars: Sequence[torch.Tensor], factors: Sequence[float],
