@@ -706,6 +706,36 @@ def clip_by_value(t, clip_value_min, clip_value_max, name=None) -> Tensor:
     return minimum(maximum(t, clip_value_min), clip_value_max, name=name or "clip_by_value")
 
 
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def newton_schulz(t, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
+                  epsilon: float = 1e-7, name=None) -> Tensor:
+    """``t`` -- a matrix, or a stack of matrices of rank 3 -- with its singular values moved
+    towards one by ``steps`` Newton-Schulz products (``X = t / (|t| + epsilon)``, then ``X = a X +
+    (b A + c A A) X`` with ``A = X X^T``): an update of equal size in every direction, between
+    ``compute_gradients`` and ``apply_gradients`` like ``clip_by_norm``. ``coefficients``: one
+    (a, b, c) or one per step. Not differentiable."""
+    t = convert_to_tensor(t)
+    if t.dtype.name not in ("float32", "bfloat16", "float16"):
+        raise TypeError("newton_schulz: fp32, bf16 or fp16 input, got %s" % t.dtype.name)
+    if t.shape is None or len(t.shape) not in (2, 3):
+        raise ValueError("newton_schulz needs a matrix or a stack of matrices, got shape %s"
+                         % (t.shape,))
+    steps = int(steps)
+    if not 1 <= steps <= 32:
+        raise ValueError("newton_schulz: steps must be 1..32, got %d" % steps)
+    rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else coefficients
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError("newton_schulz: coefficients are one (a, b, c) or one for each of the %d "
+                         "steps" % steps)
+    if not epsilon >= 0.0:
+        raise ValueError("newton_schulz: epsilon must not be negative, got %r" % (epsilon,))
+    return _op1("NewtonSchulz", [t], t.dtype, t.shape, name=name or "newton_schulz", steps=steps,
+                coefficients=tuple(tuple(float(v) for v in r) for r in rows),
+                epsilon=float(epsilon))
+
+
 # ---------------------------------------------------------------------------------------
 # control / grouping
 # ---------------------------------------------------------------------------------------

@@ -676,6 +676,12 @@ def _truncated_normal(op, inputs, ctx):
                                  op.attrs["stddev"], ctx.device)]
 
 
+@hip_kernel("NewtonSchulz")
+def _newton_schulz(op, inputs, ctx):
+    return [hip.newton_schulz(inputs[0], op.attrs["steps"], op.attrs["coefficients"],
+                              op.attrs["epsilon"])]
+
+
 def _local_f32(ctx, var_op):
     store = ctx.session._store_for(var_op)
     fast = getattr(store, "local_tensor", None)
@@ -792,7 +798,14 @@ def _optim_launch(ctx, rule, hyper, var_ops, slot_ops_list, power_ops, grads, lr
         if len(slots) > 1:
             s1.append(slots[1])
         ctx.session._store_for(var_op).update_count += 1
-    if ps:
+    if ps and rule == "muon":
+        from .ref_kernels import muon_rule
+        h, coef, _ = muon_rule(hyper, ps[0].shape)
+        hip.multi_muon(ps, [g.view(p.shape) for p, g in zip(ps, gs)], s0,
+                       h["lr"] if lr is None else lr, h["momentum"], bool(h["nesterov"]),
+                       h["weight_decay"], [muon_rule(hyper, p.shape)[2] for p in ps],
+                       int(h["steps"]), coef, h["epsilon"])
+    elif ps:
         hip.multi_optim(rule, ps, gs, s0, s1, hyper, powers, lr=lr)
     return rest
 

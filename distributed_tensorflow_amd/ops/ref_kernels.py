@@ -128,6 +128,39 @@ def _apply_sgd(op, inputs, ctx):
     return [ctx.var_apply_sgd(op.inputs[0].op, op.attrs["learning_rate"], grad)]
 
 
+def newton_schulz(g, coefficients, epsilon: float):
+    """One matrix orthogonalised in fp32 (or fp64 for an fp64 matrix), in ``g``'s dtype."""
+    x = g if g.dtype == torch.float64 else g.float()
+    if x.numel() == 0:
+        return g.clone()
+    tall = x.shape[0] > x.shape[1]
+    if tall:
+        x = x.t()
+    norm = torch.sqrt((x.double() * x.double()).sum())
+    x = (x.double() / (norm + epsilon)).to(x.dtype)
+    for a, b, c in coefficients:
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return (x.t() if tall else x).to(g.dtype).contiguous()
+
+
+# constants of the "muon" rule, in the order of ``hyper``; (a, b, c) of every step follow
+MUON_HYPER = ("lr", "momentum", "nesterov", "weight_decay", "rms_scale", "epsilon", "steps")
+
+
+def muon_rule(hyper, shape):
+    """(constants by name, coefficients per step, scale) of the "muon" rule for one variable."""
+    h = dict(zip(MUON_HYPER, hyper))
+    tail = hyper[len(MUON_HYPER):]
+    coef = [tuple(tail[3 * k:3 * k + 3]) for k in range(int(h["steps"]))]
+    rows, cols = shape[-2], shape[-1]
+    if h["rms_scale"]:
+        scale = h["rms_scale"] * math.sqrt(max(rows, cols))
+    else:
+        scale = math.sqrt(max(1.0, cols / rows)) if rows else 1.0
+    return h, coef, scale
+
+
 def optimizer_rule_step(rule: str, hyper, w, g, s0, s1=None, powers=None):
     """One step of a slot-carrying update rule on plain tensors, in fp32 (or the variable's
     dtype): returns ``(new w, new s0, new s1)``. The formulas are TensorFlow's
@@ -163,6 +196,13 @@ def optimizer_rule_step(rule: str, hyper, w, g, s0, s1=None, powers=None):
         s0 = s0 + (1.0 - b1) * (g - s0)
         s1 = s1 + (1.0 - b2) * (g * g - s1)
         w = w - lr_t * s0 / (torch.sqrt(s1) + eps)
+    elif rule == "muon":
+        h, coef, scale = muon_rule(hyper, tuple(w.shape))
+        s0 = h["momentum"] * s0 + g
+        u = g + h["momentum"] * s0 if h["nesterov"] else s0
+        o = torch.stack([newton_schulz(m, coef, h["epsilon"]) for m in u]) if u.dim() == 3 \
+            else newton_schulz(u, coef, h["epsilon"])
+        w = (1.0 - h["lr"] * h["weight_decay"]) * w - (h["lr"] * scale) * o
     else:
         raise ValueError("unknown optimizer rule %r" % (rule,))
     return w, s0, s1
@@ -218,6 +258,14 @@ def affine_through_store(ctx, var_op, factor: float, increment: float):
     if getattr(store, "local_tensor", lambda n: None)(var_op.name) is not None:
         return ctx.var_assign(var_op, new)
     return ctx.var_assign_add(var_op, new - cur)
+
+
+@ref_kernel("NewtonSchulz")
+def _newton_schulz(op, inputs, ctx):
+    g, coef, eps = inputs[0], op.attrs["coefficients"], op.attrs["epsilon"]
+    if g.dim() == 2:
+        return [newton_schulz(g, coef, eps)]
+    return [torch.stack([newton_schulz(m, coef, eps) for m in g]) if len(g) else g.clone()]
 
 
 @ref_kernel("AffineUpdateVariable", stateful=True)

@@ -1,6 +1,6 @@
 """Optimizers: ``GradientDescentOptimizer(lr).minimize(loss, global_step=...)`` and the
 slot-carrying rules of the same family (``MomentumOptimizer``, ``AdagradOptimizer``,
-``RMSPropOptimizer``, ``AdamOptimizer``).
+``RMSPropOptimizer``, ``AdamOptimizer``), and ``MuonOptimizer`` for weight matrices.
 
 Reference usage: ``tf_distributed.py:75-76``. ``minimize`` = ``compute_gradients``
 (reverse-mode autodiff) + ``apply_gradients`` (one ``ApplyGradientDescent`` per variable,
@@ -96,7 +96,7 @@ class Optimizer:
         return self._slots
 
     def _zeros_slot(self, var: Variable, slot_name: str, op_name: str,
-                    value: float = 0.0) -> Variable:
+                    value: float = 0.0, per_element: bool = True) -> Variable:
         slots = self._slot_dict().setdefault(slot_name, {})
         if var not in slots:
             g = var.graph
@@ -105,10 +105,11 @@ class Optimizer:
                 slots[var] = Variable(
                     F.fill(tuple(var.shape), value, dtype=var.dtype), trainable=False,
                     name=var.op.name + "/" + op_name)
-            # per-element state of `var`: a runtime that gives every parameter shard one owner
-            # (reduce_scatter_sync) keeps only the owner's part of it
-            slots[var].op.attrs["slot_of"] = var.op.name
-            slots[var].op.attrs["slot_key"] = op_name
+            if per_element:
+                # a runtime that gives every parameter shard one owner (reduce_scatter_sync)
+                # keeps only the owner's part of it
+                slots[var].op.attrs["slot_of"] = var.op.name
+                slots[var].op.attrs["slot_key"] = op_name
         return slots[var]
 
     def get_slot(self, var: Variable, name: str) -> Optional[Variable]:
@@ -289,6 +290,80 @@ class AdamOptimizer(Optimizer):
                     name="advance_" + power.op.name.split("/")[-1],
                     attrs={"factor": beta, "increment": 0.0}))
         return out
+
+
+class MuonOptimizer(Optimizer):
+    """Momentum whose update is orthogonalised, for the matrices of dense layers: ``v = momentum *
+    v + grad; u = grad + momentum * v`` (``use_nesterov``; else ``v``); ``var = (1 - lr *
+    weight_decay) * var - lr * s * newton_schulz(u)``.
+
+    ``s`` is ``sqrt(max(1, outputs / inputs))`` for a variable of [inputs, outputs], or with
+    ``rms_scale`` (0.2 gives updates of the size Adam's have) ``rms_scale * sqrt(max(inputs,
+    outputs))``. Variables of rank 2, and of rank 3 as stacks of matrices, follow the rule;
+    ``vector_optimizer`` updates all others (biases, layer-norm parameters), and without one they
+    are refused. ``steps``, ``coefficients`` and ``epsilon``: see ``tf.newton_schulz``. The rule
+    needs whole matrices, so under ``reduce_scatter_sync`` its variables take the all-reduce path
+    and their momentum is replicated."""
+
+    def __init__(self, learning_rate, momentum: float = 0.95, use_nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5,
+                 coefficients=F.NEWTON_SCHULZ_COEFFICIENTS, epsilon: float = 1e-7,
+                 rms_scale: float = 0.0, vector_optimizer: Optional[Optimizer] = None,
+                 use_locking: bool = False, name: str = "Muon"):
+        super().__init__(use_locking, name)
+        self._learning_rate, self._lr_tensor = self._split_lr(learning_rate)
+        steps = int(steps)
+        if not 1 <= steps <= 32:
+            raise ValueError("steps must be 1..32, got %d" % steps)
+        rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else coefficients
+        if len(rows) != steps or any(len(r) != 3 for r in rows):
+            raise ValueError("coefficients are one (a, b, c) or one for each of the %d steps"
+                             % steps)
+        if not epsilon >= 0.0 or rms_scale < 0.0:
+            raise ValueError("epsilon and rms_scale must not be negative")
+        # (the order of ref_kernels.MUON_HYPER)
+        self._hyper = (self._learning_rate, float(momentum), float(bool(use_nesterov)),
+                       float(weight_decay), float(rms_scale), float(epsilon), float(steps),
+                       *[float(v) for r in rows for v in r])
+        self._vector_optimizer = vector_optimizer
+
+    @staticmethod
+    def _is_matrix(var: Variable) -> bool:
+        return var.shape is not None and len(var.shape) in (2, 3)
+
+    def _create_slots(self, var_list):
+        vectors = [v for v in var_list if not self._is_matrix(v)]
+        if vectors and self._vector_optimizer is None:
+            raise ValueError("MuonOptimizer orthogonalises matrices; give a vector_optimizer for "
+                             "%s" % ", ".join(v.op.name for v in vectors))
+        for v in var_list:
+            if self._is_matrix(v):
+                self._zeros_slot(v, "momentum", self._name, per_element=False)
+        self._has_vectors = bool(vectors)
+        if vectors:
+            self._vector_optimizer._create_slots(vectors)
+
+    def _apply_dense(self, grad, var):
+        if not self._is_matrix(var):
+            return self._vector_optimizer._apply_dense(grad, var)
+        return self._apply_rule("muon", self._hyper, var, [self.get_slot(var, "momentum")], grad,
+                                self._lr_tensor)
+
+    def _finish(self, updates):
+        return self._vector_optimizer._finish(updates) if self._has_vectors else []
+
+    def get_slot(self, var, name):
+        slot = super().get_slot(var, name)
+        if slot is None and self._vector_optimizer is not None:
+            slot = self._vector_optimizer.get_slot(var, name)
+        return slot
+
+    def get_slot_names(self):
+        """The matrices' slot first, then those of the vector optimizer."""
+        names = super().get_slot_names()
+        if self._vector_optimizer is not None:
+            names += [n for n in self._vector_optimizer.get_slot_names() if n not in names]
+        return names
 
 
 class SyncReplicasOptimizer(Optimizer):
