@@ -28,19 +28,28 @@
 // the LDS image of a 64-element bf16 K-tile (16-byte pieces, XOR-swizzled by row) and lands there
 // by 16-byte LDS-DMA. Rows are padded with zeros to whole chunks; edge tiles read the last row
 // again instead of rows that are not there.
-#include "common.h"
+#include "elem.h"
 
 namespace {
 
+constexpr int NS_CHAIN = 4;            // K-tiles an accumulator runs through before it is emptied
 constexpr int NS_MAX_MATS = 16;
 constexpr int NS_MAX_STEPS = 32;
-constexpr int NS_MAX_PARTS = 512;      // workgroups that share a matrix's sum of squares
+constexpr int NS_SLOTS = 512;          // workgroups of a product that run at once: two per CU
+constexpr int NS_MAX_PARTS = 1024;     // workgroups that share a matrix's sum of squares
 constexpr float X_SCALE = 16384.f, AB_SCALE = 4096.f;
 constexpr double X_LIMIT = 3.5, AB_LIMIT = 15.0;   // times the scales: below fp16's 65504
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+struct yes {
+  static constexpr bool value = true;
+};
+struct no {
+  static constexpr bool value = false;
+};
 
 enum { NS_F32 = 0, NS_BF16 = 1, NS_F16 = 2 };
 enum { TO_A = 0, TO_B = 1, TO_X = 2, TO_OUT = 3 };
@@ -63,8 +72,13 @@ struct NsMat {
 };
 struct NsArgs {
   NsMat t[NS_MAX_MATS];
-  int first[NS_MAX_MATS + 1];    // first workgroup of each matrix in this launch
+  int first[NS_MAX_MATS + 1];    // first tile (or workgroup) of each matrix in this launch
   int count;
+  // products: tiles [0, unsplit) have a workgroup each; every later tile has `splits`
+  // workgroups that share its K range
+  int unsplit, splits;
+  float* partial;                // [(tile - unsplit) * splits + split][T * T]
+  int* arrived;                  // [tile - unsplit], zero between launches
 };
 struct NsMuon {
   const float* lr_dev;
@@ -76,17 +90,6 @@ __device__ __forceinline__ int matrix_of(const NsArgs& args, int id) {
   int i = 0;
   while (i + 1 < args.count && id >= args.first[i + 1]) ++i;
   return i;
-}
-
-__device__ __forceinline__ float ns_load(const void* p, long i, int type) {
-  if (type == NS_F32) return ((const float*)p)[i];
-  if (type == NS_BF16) return dtf_bf16_to_f32(((const unsigned short*)p)[i]);
-  return (float)((const _Float16*)p)[i];
-}
-__device__ __forceinline__ void ns_store(void* p, long i, int type, float v) {
-  if (type == NS_F32) ((float*)p)[i] = v;
-  else if (type == NS_BF16) ((unsigned short*)p)[i] = dtf_f32_to_bf16(v);
-  else ((_Float16*)p)[i] = (_Float16)v;
 }
 
 // hi | lo << 16
@@ -114,21 +117,32 @@ __device__ __forceinline__ long split_off(int c) { return (long)(c >> 5) * 128 +
 
 // ---- momentum and sum of squares -------------------------------------------------------------
 // Squares are summed in 64 bits: gradients of 1e-20 or 1e+25 have squares fp32 does not hold.
-template <bool MUON>
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs args, int type, NsMuon mo) {
+template <typename E, bool MUON>
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs args, NsMuon mo) {
+  constexpr int V = 16 / (int)sizeof(E);
   const int mat = matrix_of(args, blockIdx.x);
   const NsMat& t = args.t[mat];
   const int part = blockIdx.x - args.first[mat];
-  const long total = (long)t.rows * t.cols;
+  const long total = (long)t.rows * t.cols, stride = t.nparts * 256L * V;
+  const E* g = (const E*)t.g;
   double s = 0.0;
-  for (long i = part * 256L + threadIdx.x; i < total; i += t.nparts * 256L) {
-    float u = ns_load(t.g, i, type);
+#pragma unroll 4
+  for (long i = (part * 256L + threadIdx.x) * V; i < total; i += stride) {
+    const int n = total - i < V ? (int)(total - i) : V;
+    float u[V];
+    load_part<V>(g + i, 0, n, u);
     if (MUON) {
-      const float v = __builtin_fmaf(mo.mu, t.v[i], u);
-      t.v[i] = v;
-      u = mo.nesterov ? __builtin_fmaf(mo.mu, v, u) : v;
+      float v[V];
+      load_part<V>(t.v + i, 0, n, v);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        v[k] = __builtin_fmaf(mo.mu, v[k], u[k]);
+        u[k] = mo.nesterov ? __builtin_fmaf(mo.mu, v[k], u[k]) : v[k];
+      }
+      store_part<V>(t.v + i, 0, n, v);
     }
-    s = __builtin_fma((double)u, (double)u, s);
+#pragma unroll
+    for (int k = 0; k < V; ++k) s = __builtin_fma((double)u[k], (double)u[k], s);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
@@ -136,21 +150,38 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs args, int type, NsM
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) t.parts[part] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < NS_SLOTS; i += 256) args.arrived[i] = 0;
 }
 
 // ---- X and its transpose in split rows -------------------------------------------------------
 // One 64 x 64 tile of G per workgroup: its rows go to one of the two orders as they are, its
 // columns through LDS to the other.
-template <bool MUON>
-__global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, int type, float eps,
-                                                       NsMuon mo) {
-  __shared__ unsigned tr[64 * 68];
+template <typename E, bool MUON>
+__global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, float eps, NsMuon mo) {
+  // (rows of 65 dwords: the 8 x 8 lanes of a wave meet 64 banks both ways)
+  __shared__ unsigned tr[64 * 65];
   __shared__ double sh[4];
   const int mat = matrix_of(args, blockIdx.x);
   const NsMat& t = args.t[mat];
   const int tile = blockIdx.x - args.first[mat];
   const int tiles_c = (t.cols + 63) / 64;
   const int r0 = tile / tiles_c * 64, c0 = tile % tiles_c * 64;
+  const int c8 = (threadIdx.x & 7) * 8, c = c0 + c8;
+  float u[2][8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = r0 + (threadIdx.x >> 3) + 32 * h;
+    const int n = r < t.rows ? t.cols : 0;
+    const long at = (long)(r < t.rows ? r : 0) * t.cols;
+    load_part<8>((const E*)t.g + at, c, n, u[h]);
+    if (MUON) {
+      float v[8];                                  // already advanced
+      load_part<8>(t.v + at, c, n, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[h][k] = mo.nesterov ? __builtin_fmaf(mo.mu, v[k], u[h][k]) : v[k];
+    }
+  }
   double s = 0.0;
   for (int p = threadIdx.x; p < t.nparts; p += 256) s += t.parts[p];
 #pragma unroll
@@ -165,25 +196,15 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, int type, fl
   char* turned = tall ? t.x : t.xt0;               // rows of `rows` elements
   const long direct_pitch = 4L * (tall ? t.km : t.kn);
   const long turned_pitch = 4L * (tall ? t.kn : t.km);
-  const int c8 = (threadIdx.x & 7) * 8, c = c0 + c8;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int rl = (threadIdx.x >> 3) + 32 * h, r = r0 + rl;
     unsigned p[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      float u = 0.f;
-      if (r < t.rows && c + k < t.cols) {
-        const long i = (long)r * t.cols + c + k;
-        u = ns_load(t.g, i, type);
-        if (MUON) {
-          const float v = t.v[i];                  // already advanced
-          u = mo.nesterov ? __builtin_fmaf(mo.mu, v, u) : v;
-        }
-        u = (float)((double)u * mul);
-      }
-      p[k] = split_pack(u);
-      tr[(c8 + k) * 68 + rl] = p[k];
+      // (0 / 0 of a zero matrix without epsilon stays in the matrix: padding is zero always)
+      p[k] = r < t.rows && c + k < t.cols ? split_pack((float)((double)u[h][k] * mul)) : 0u;
+      tr[(c8 + k) * 65 + rl] = p[k];
     }
     // (a chunk that starts inside the row belongs to it as a whole)
     if (r < t.rows && (c & ~31) < t.cols) store_split8(direct + r * direct_pitch + split_off(c), p);
@@ -195,7 +216,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, int type, fl
     if (c0 + cl < t.cols && ((r0 + c8) & ~31) < t.rows) {
       unsigned p[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) p[k] = tr[cl * 68 + c8 + k];
+      for (int k = 0; k < 8; ++k) p[k] = tr[cl * 65 + c8 + k];
       store_split8(turned + (c0 + cl) * turned_pitch + split_off(r0 + c8), p);
     }
   }
@@ -206,26 +227,56 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const char* base) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0xffffffff, 0x00020000);
 }
 
+// workgroups that share a K range of kt K-tiles when `most` are offered: at least 8 each
+__host__ __device__ __forceinline__ int split_count(int kt, int most) {
+  const int fit = kt / 8;
+  return fit < 1 ? 1 : fit < most ? fit : most;
+}
+
 // byte offset of 16-byte piece kc of a row inside an operand tile (rows of 128 bytes)
 __device__ __forceinline__ int piece_off(int row, int kc) {
   return row * 128 + ((kc ^ ((row >> 1) & 7)) << 4);
 }
 
 // One T x T tile of P Q^T, P [M][K] and Q [N][K] in split rows, by four waves of T/2 x T/2.
-// Two K-tile buffers: the requests for the next K-tile are in flight while this one multiplies.
 // TO_A / TO_B: symmetric results (M = N, tiles on and below the diagonal), written to both
 // places; TO_X: written in both orders; TO_OUT: the caller's type.
-template <int T, int TO, bool MUON>
-__device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, int type, float ca,
-                                                float cb, float cc, const NsMuon& mo) {
+//
+// K loop. WS: four more waves issue the LDS-DMA requests, NB - 1 K-tiles ahead into NB buffers,
+// so that the multiplying waves never wait at the address unit. Otherwise two buffers, and a
+// second workgroup on the CU covers the waits.
+//
+// Accumulation. The matrix instruction adds its 32 products to the accumulator in steps of its
+// own; a long chain of them loses more than fp32 sums of rounded products do (1024 x 1024: the
+// result was off by 4.7e-6, an fp32 computation by 3.1e-6). Every NS_CHAIN K-tiles the
+// accumulators are added to a second set and start again from zero.
+//
+// Splits. A tile whose K range is shared leaves fp32 partial tiles in memory; the workgroup that
+// arrives last adds all of them in split order, whoever it is, so the bits do not depend on the
+// order of arrival.
+template <typename E, int T, int TO, bool MUON, bool WS>
+__device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, float ca, float cb,
+                                                float cc, const NsMuon& mo) {
   constexpr int NI = T / 32;                    // 16 x 16 tiles per wave and direction
   constexpr int WT = T / 2;
   constexpr int OP_BYTES = T * 128, BUF_BYTES = 2 * OP_BYTES;
+  constexpr int NB = WS ? 4 : 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = wave8 & 3;
+  const bool producer = WS && wave8 >= 4;
   const int wr = wave >> 1, wc = wave & 1;
-  const int id = dtf_xcd_remap(blockIdx.x, gridDim.x);
+  int id, split = 0, splits = 1;
+  if ((int)blockIdx.x < args.unsplit) {
+    id = dtf_xcd_remap(blockIdx.x, args.unsplit);
+  } else {
+    const int r = blockIdx.x - args.unsplit;
+    splits = args.splits;
+    id = args.unsplit + r / splits;
+    split = r % splits;
+  }
+  const int shared_tile = id - args.unsplit;
   const int mat = matrix_of(args, id);
   const NsMat& t = args.t[mat];
   const int tile = id - args.first[mat];
@@ -246,6 +297,13 @@ __device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, in
       P = t.b; Q = xt; M = t.m; N = t.n;
     }
   }
+  const int all_kt = K / 32;
+  if (splits > 1) {                             // (a matrix with a short K uses fewer)
+    splits = split_count(all_kt, splits);
+    if (split >= splits) return;
+  }
+  const int kt0 = (int)((long)all_kt * split / splits);
+  const int nkt = (int)((long)all_kt * (split + 1) / splits) - kt0;
   int tm, tn;
   if (TO == TO_A || TO == TO_B) {
     tm = (int)((__builtin_sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
@@ -285,40 +343,138 @@ __device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, in
     }
   };
 
-  f32x4 acc[NI][NI];
+  f32x4 sum[NI][NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NI; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int frow = lane & 15, fq = lane >> 4;
-  const int nkt = K / 32;
-  request(0, smem);
-  for (int kt = 0; kt < nkt; ++kt) {
-    // K-tile kt has landed for every wave, and every wave is done with the other buffer
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    const char* cur = smem + (kt & 1) * BUF_BYTES;
-    if (kt + 1 < nkt) request(kt + 1, smem + ((kt + 1) & 1) * BUF_BYTES);
-    f16x8 ph[NI], pl[NI], qh[NI], ql[NI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int rp = wr * WT + i * 16 + frow, rq = wc * WT + i * 16 + frow;
-      ph[i] = *reinterpret_cast<const f16x8*>(cur + piece_off(rp, fq));
-      pl[i] = *reinterpret_cast<const f16x8*>(cur + piece_off(rp, 4 + fq));
-      qh[i] = *reinterpret_cast<const f16x8*>(cur + OP_BYTES + piece_off(rq, fq));
-      ql[i] = *reinterpret_cast<const f16x8*>(cur + OP_BYTES + piece_off(rq, 4 + fq));
+  if (WS && producer) {
+    constexpr int R = 2 * NI;                   // requests per wave and K-tile
+    for (int kt = 0; kt < NB - 1 && kt < nkt; ++kt) request(kt0 + kt, smem + kt * BUF_BYTES);
+    for (int kt = 0; kt < nkt; ++kt) {
+      // own pieces of K-tile kt have landed; those of up to NB - 2 later ones stay in flight
+      if (nkt - 1 - kt >= 2)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * R) : "memory");
+      else if (nkt - 1 - kt == 1)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_barrier" ::: "memory");
+      // behind the barrier the multiplying waves are done with the buffer of K-tile kt - 1
+      if (kt + NB - 1 < nkt) request(kt0 + kt + NB - 1, smem + (kt + NB - 1) % NB * BUF_BYTES);
     }
+    asm volatile("s_barrier" ::: "memory");
+    if (splits == 1) return;
+  } else {
+    if (!WS) request(kt0, smem);
+    f32x4 acc[NI][NI];
+    // one K-tile; FIRST: the accumulators start from zero
+    auto multiply = [&](int kt, auto first) {
+      constexpr bool FIRST = decltype(first)::value;
+      // K-tile kt has landed for every wave, and every wave is done with the buffer before it
+      if (WS) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (kt + 1 < nkt) request(kt0 + kt + 1, smem + ((kt + 1) & 1) * BUF_BYTES);
+      }
+      const char* cur = smem + kt % NB * BUF_BYTES;
+      f16x8 ph[NI], pl[NI], qh[NI], ql[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int rp = wr * WT + i * 16 + frow, rq = wc * WT + i * 16 + frow;
+        ph[i] = *reinterpret_cast<const f16x8*>(cur + piece_off(rp, fq));
+        pl[i] = *reinterpret_cast<const f16x8*>(cur + piece_off(rp, 4 + fq));
+        qh[i] = *reinterpret_cast<const f16x8*>(cur + OP_BYTES + piece_off(rq, fq));
+        ql[i] = *reinterpret_cast<const f16x8*>(cur + OP_BYTES + piece_off(rq, 4 + fq));
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          // (operands swapped: a lane's four results lie along N)
+          const f32x4 from = FIRST ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j];
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph[i], from, 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl[i], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph[i], acc[i][j], 0, 0, 0);
+        }
+    };
+    for (int base = 0; base < nkt; base += NS_CHAIN) {
+      multiply(base, yes());
+      const int end = base + NS_CHAIN < nkt ? base + NS_CHAIN : nkt;
+      for (int kt = base + 1; kt < end; ++kt) multiply(kt, no());
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) sum[i][j] += acc[i][j];
+    }
+    // the buffers become the epilogue's scratch
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+
+  if (splits > 1) {
+    __shared__ int last;
+    constexpr int PAIRS = T * T / 2;            // 8-byte pairs in a partial tile
+    typedef unsigned long long pair_t;
+    pair_t* mine = reinterpret_cast<pair_t*>(args.partial) +
+                   ((long)shared_tile * args.splits + split) * PAIRS + (tid & 255);
+    // The XCDs' L2s do not see each other's lines, so the parts go through memory: stores and
+    // loads of device scope pass the L2 by, and a store is complete once it has arrived there.
+    // (A release fence instead writes the whole L2 back, 0.4 us each and one after the other on
+    // an XCD: 29 us for this product at 1024 x 1024.)
+    if (!producer) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const pair_t v = (pair_t)__float_as_uint(sum[i][j][2 * h]) |
+                             (pair_t)__float_as_uint(sum[i][j][2 * h + 1]) << 32;
+            __hip_atomic_store(mine + ((i * NI + j) * 2 + h) * 256, v, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+          }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's part has arrived ...
+    __syncthreads();                                   // ... and every wave's, before the count
+    if (tid == 0) {
+      const int before = __hip_atomic_fetch_add(&args.arrived[shared_tile], 1, __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT);
+      last = before == splits - 1;
+      if (last)                                 // nobody else comes: ready for the next launch
+        __hip_atomic_store(&args.arrived[shared_tile], 0, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last || producer) return;
+    pair_t* all = reinterpret_cast<pair_t*>(args.partial) +
+                  (long)shared_tile * args.splits * PAIRS + tid;
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        // (operands swapped: a lane's four results lie along N)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph[i], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl[i], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph[i], acc[i][j], 0, 0, 0);
-      }
+      for (int j = 0; j < NI; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < splits; ++k) {
+      pair_t v[NI][NI][2];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            v[i][j][h] = __hip_atomic_load(all + ((i * NI + j) * 2 + h) * 256, __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            sum[i][j][r] += __uint_as_float((unsigned)(v[i][j][r >> 1] >> (32 * (r & 1))));
+      all += PAIRS;
+    }
   }
-  __syncthreads();                              // the buffers become the epilogue's scratch
+  auto& acc = sum;
 
   // lane: rows mb + 16 i, columns nb + 16 j + 0..3
   const int mb = m0 + wr * WT + frow, nb = n0 + wc * WT + 4 * fq;
@@ -329,21 +485,20 @@ __device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, in
     for (int i = 0; i < NI; ++i) {
       const int m = mb + 16 * i;
       if (m >= M) continue;
+      E* row = (E*)t.out + (long)m * N;
 #pragma unroll
-      for (int j = 0; j < NI; ++j)
+      for (int j = 0; j < NI; ++j) {
+        const int n = nb + 16 * j;
+        if (n >= N) continue;
+        float v[4], w[4];
+        if (MUON) load_part<4>(row, n, N, w);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int n = nb + 16 * j + r;
-          if (n >= N) continue;
-          const long at = (long)m * N + n;
-          const float v = acc[i][j][r] * (1.f / (X_SCALE * AB_SCALE));
-          if (MUON) {
-            float* w = (float*)t.out;
-            w[at] = __builtin_fmaf(-take, v, keep * w[at]);
-          } else {
-            ns_store(t.out, at, type, v);
-          }
+          v[r] = acc[i][j][r] * (1.f / (X_SCALE * AB_SCALE));
+          if (MUON) v[r] = __builtin_fmaf(-take, v[r], keep * w[r]);
         }
+        store_part<4>(row, n, N, v);
+      }
     }
     return;
   }
@@ -376,8 +531,8 @@ __device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, in
         pk[i][j][r] = m < M && n + r < N ? split_pack(v[r]) : 0u;
     }
 
-  char* D = TO == TO_A ? t.a : TO == TO_B ? t.b : t.x;          // rows along M
-  char* E = TO == TO_X ? ((step & 1) ? t.xt0 : t.xt1) : D;      // rows along N
+  char* direct = TO == TO_A ? t.a : TO == TO_B ? t.b : t.x;          // rows along M
+  char* turned = TO == TO_X ? ((step & 1) ? t.xt0 : t.xt1) : direct;   // rows along N
   const long d_pitch = 4L * (TO == TO_X ? t.kn : t.km), e_pitch = 4L * t.km;
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -385,7 +540,7 @@ __device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, in
     for (int j = 0; j < NI; ++j) {
       const int m = mb + 16 * i, n = nb + 16 * j;
       if (m < M && (n & ~31) < N) {
-        char* dst = D + m * d_pitch + split_off(n);
+        char* dst = direct + m * d_pitch + split_off(n);
         const unsigned* p = pk[i][j];
         *reinterpret_cast<uint2*>(dst) = uint2{(p[0] & 0xffffu) | p[1] << 16,
                                                (p[2] & 0xffffu) | p[3] << 16};
@@ -414,16 +569,17 @@ __device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, in
       const u32x4* src = reinterpret_cast<const u32x4*>(strip + nl * 36 + (lane & 3) * 8);
       *reinterpret_cast<u32x4*>(p) = src[0];
       *reinterpret_cast<u32x4*>(p + 4) = src[1];
-      if (n < N && mc < M) store_split8(E + n * e_pitch + split_off(mc + (lane & 3) * 8), p);
+      if (n < N && mc < M) store_split8(turned + n * e_pitch + split_off(mc + (lane & 3) * 8), p);
     }
     __builtin_amdgcn_wave_barrier();
   }
 }
 
-template <int T, int TO, bool MUON>
-__global__ __launch_bounds__(256) void ns_product_kernel(NsArgs args, int step, int type,
-                                                         float ca, float cb, float cc, NsMuon mo) {
-  ns_product_body<T, TO, MUON>(args, step, type, ca, cb, cc, mo);
+// 64 x 64 tiles: with request-issuing waves; 128 x 128: without. Two workgroups per CU either way.
+template <typename E, int T, int TO, bool MUON>
+__global__ __launch_bounds__(T == 64 ? 512 : 256, T == 64 ? 4 : 2) void ns_product_kernel(
+    NsArgs args, int step, float ca, float cb, float cc, NsMuon mo) {
+  ns_product_body<E, T, TO, MUON, T == 64>(args, step, ca, cb, cc, mo);
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -479,40 +635,80 @@ void allow_lds(KernelT kernel, int lds) {
   (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
 }
 
-template <int T, bool MUON>
-int launch_steps(NsArgs& args, int type, int steps, const float* coef, const NsMuon& mo,
+// Which tiles of a product are split along K: those behind the last full round of the chip, as
+// many ways as the round has workgroups for.
+void plan_splits(NsArgs& args, int kt_max) {
+  const int tiles = args.first[args.count];
+  args.unsplit = tiles / NS_SLOTS * NS_SLOTS;
+  const int rest = tiles - args.unsplit;
+  args.splits = rest ? split_count(kt_max, NS_SLOTS / rest < 16 ? NS_SLOTS / rest : 16) : 1;
+  if (args.splits == 1) args.unsplit = tiles;
+}
+unsigned grid_of(const NsArgs& args) {
+  return args.unsplit + (args.first[args.count] - args.unsplit) * args.splits;
+}
+
+template <typename E, int T, bool MUON>
+int launch_steps(const NsArgs& args, int steps, const float* coef, const NsMuon& mo,
                  hipStream_t stream) {
-  constexpr int LDS = 2 * 2 * T * 128;
+  constexpr int LDS = (T == 64 ? 4 : 2) * 2 * T * 128;
   static_assert(4 * (T / 2) * 36 * 4 <= LDS, "the epilogue's strips fit the K-tile buffers");
   static DtfPerDeviceOnce once;
   dtf_once_per_device(once, [&] {
-    allow_lds(ns_product_kernel<T, TO_A, false>, LDS);
-    allow_lds(ns_product_kernel<T, TO_B, false>, LDS);
-    allow_lds(ns_product_kernel<T, TO_X, false>, LDS);
-    allow_lds(ns_product_kernel<T, TO_OUT, MUON>, LDS);
+    allow_lds(ns_product_kernel<float, T, TO_A, false>, LDS);
+    allow_lds(ns_product_kernel<float, T, TO_B, false>, LDS);
+    allow_lds(ns_product_kernel<float, T, TO_X, false>, LDS);
+    allow_lds(ns_product_kernel<E, T, TO_OUT, MUON>, LDS);
   });
   NsArgs sym = args, full = args;
+  int km = 0, kn = 0;
   for (int i = 0; i < args.count; ++i) {
     const int tm = (args.t[i].m + T - 1) / T, tn = (args.t[i].n + T - 1) / T;
     sym.first[i + 1] = sym.first[i] + tm * (tm + 1) / 2;
     full.first[i + 1] = full.first[i] + tm * tn;
+    km = args.t[i].km > km ? args.t[i].km : km;
+    kn = args.t[i].kn > kn ? args.t[i].kn : kn;
   }
-  const dim3 gs(sym.first[args.count]), gf(full.first[args.count]), block(256);
+  NsArgs square = sym;
+  plan_splits(sym, kn / 32);
+  plan_splits(square, km / 32);
+  plan_splits(full, km / 32);
+  const dim3 block(T == 64 ? 512 : 256);
   for (int k = 0; k < steps; ++k) {
     const float a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
-    hipLaunchKernelGGL((ns_product_kernel<T, TO_A, false>), gs, block, LDS, stream, sym, k, type,
-                       a, b, c, mo);
-    hipLaunchKernelGGL((ns_product_kernel<T, TO_B, false>), gs, block, LDS, stream, sym, k, type,
-                       a, b, c, mo);
+    hipLaunchKernelGGL((ns_product_kernel<float, T, TO_A, false>), dim3(grid_of(sym)), block, LDS, stream,
+                       sym, k, a, b, c, mo);
+    hipLaunchKernelGGL((ns_product_kernel<float, T, TO_B, false>), dim3(grid_of(square)), block, LDS,
+                       stream, square, k, a, b, c, mo);
     if (k + 1 < steps)
-      hipLaunchKernelGGL((ns_product_kernel<T, TO_X, false>), gf, block, LDS, stream, full, k,
-                         type, a, b, c, mo);
+      hipLaunchKernelGGL((ns_product_kernel<float, T, TO_X, false>), dim3(grid_of(full)), block, LDS,
+                         stream, full, k, a, b, c, mo);
     else
-      hipLaunchKernelGGL((ns_product_kernel<T, TO_OUT, MUON>), gf, block, LDS, stream, full, k,
-                         type, a, b, c, mo);
+      hipLaunchKernelGGL((ns_product_kernel<E, T, TO_OUT, MUON>), dim3(grid_of(full)), block, LDS,
+                         stream, full, k, a, b, c, mo);
   }
   DTF_LAUNCH_CHECK();
   return DTF_OK;
+}
+
+// tile size of a call: 128 once that many tiles give the chip's 256 CUs two workgroups each
+int tile_of(long tiles128) { return tiles128 >= NS_SLOTS ? 128 : 64; }
+
+// head of the workspace: arrival counts, then the partial tiles of one split product
+constexpr long NS_HEAD = 4L * NS_SLOTS;
+long shared_bytes(int tile) { return NS_HEAD + 4L * NS_SLOTS * tile * tile; }
+
+template <typename E, bool MUON>
+int launch(const NsArgs& args, const NsArgs& parts, const NsArgs& split, int tile, int steps,
+           const float* coef, float eps, const NsMuon& mo, hipStream_t stream) {
+  const int n = args.count;
+  hipLaunchKernelGGL((ns_norm_kernel<E, MUON>), dim3(parts.first[n]), dim3(256), 0, stream, parts,
+                     mo);
+  hipLaunchKernelGGL((ns_split_kernel<E, MUON>), dim3(split.first[n]), dim3(256), 0, stream, split,
+                     eps, mo);
+  DTF_LAUNCH_CHECK();
+  return tile == 128 ? launch_steps<E, 128, MUON>(args, steps, coef, mo, stream)
+                     : launch_steps<E, 64, MUON>(args, steps, coef, mo, stream);
 }
 
 template <bool MUON>
@@ -530,9 +726,18 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
   char* at = (char*)workspace;
   long used = 0, tiles128 = 0;
   if ((uintptr_t)at & 255) return DTF_ERR_BAD_ARG;
+  for (int i = 0; i < count; ++i) {
+    if (bad_shape(rows[i], cols[i])) return DTF_ERR_BAD_ARG;
+    tiles128 += ((rows[i] + 127L) / 128) * ((cols[i] + 127L) / 128);
+  }
+  const int tile = tile_of(tiles128);
+  args.arrived = (int*)at;
+  args.partial = (float*)(at + NS_HEAD);
+  at += shared_bytes(tile);
+  used = shared_bytes(tile);
   NsArgs parts, split;
   for (int i = 0; i < count; ++i) {
-    if (bad_shape(rows[i], cols[i]) || !g[i] || !out[i] || (MUON && (!v[i])))
+    if (!g[i] || !out[i] || (MUON && (!v[i])))
       return DTF_ERR_BAD_ARG;
     const NsSizes s = sizes_of(rows[i], cols[i]);
     NsMat& t = args.t[i];
@@ -561,7 +766,6 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     at += s.sq;
     t.b = at;
     at += s.sq;
-    tiles128 += ((s.m + 127) / 128) * ((s.n + 127) / 128);
   }
   parts = split = args;
   for (int i = 0; i < count; ++i) {
@@ -570,14 +774,18 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     parts.first[i + 1] = parts.first[i] + args.t[i].nparts;
     split.first[i + 1] = split.first[i] + (int)tiles;
   }
-  hipLaunchKernelGGL((ns_norm_kernel<MUON>), dim3(parts.first[count]), dim3(256), 0, stream, parts,
-                     type, mo);
-  hipLaunchKernelGGL((ns_split_kernel<MUON>), dim3(split.first[count]), dim3(256), 0, stream,
-                     split, type, eps, mo);
-  DTF_LAUNCH_CHECK();
-  // 128 x 128 tiles once they give the chip's 256 CUs two workgroups each
-  return tiles128 >= 512 ? launch_steps<128, MUON>(args, type, steps, coef, mo, stream)
-                         : launch_steps<64, MUON>(args, type, steps, coef, mo, stream);
+  switch (type) {
+    case NS_F32: return launch<float, MUON>(args, parts, split, tile, steps, coef, eps, mo, stream);
+    case NS_BF16:
+      if constexpr (!MUON)
+        return launch<dtf_bf16, false>(args, parts, split, tile, steps, coef, eps, mo, stream);
+      break;
+    default:
+      if constexpr (!MUON)
+        return launch<_Float16, false>(args, parts, split, tile, steps, coef, eps, mo, stream);
+      break;
+  }
+  return DTF_ERR_BAD_ARG;
 }
 
 }  // namespace
@@ -585,12 +793,13 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
 // bytes of workspace (256-byte aligned) for `count` matrices; 0 for shapes that are not taken
 DTF_API long dtf_newton_schulz_workspace(int count, const int* rows, const int* cols) {
   if (count < 0 || count > NS_MAX_MATS || (count > 0 && (!rows || !cols))) return 0;
-  long total = 256;
+  long total = 256, tiles128 = 0;
   for (int i = 0; i < count; ++i) {
     if (bad_shape(rows[i], cols[i])) return 0;
+    tiles128 += ((rows[i] + 127L) / 128) * ((cols[i] + 127L) / 128);
     total += sizes_of(rows[i], cols[i]).total;
   }
-  return total;
+  return total + shared_bytes(tile_of(tiles128));
 }
 
 // out[i] = orthogonalised g[i], both [rows[i], cols[i]] contiguous of `type` (0 fp32, 1 bf16,
