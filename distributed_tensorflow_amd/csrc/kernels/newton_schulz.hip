@@ -69,6 +69,8 @@ struct NsMat {
   int km, kn;          // m, n rounded up to whole chunks
   int nparts;
   float scale;         // Muon: s
+  double* gram;        // thin matrices: [slabs][lower 16 x 16 tiles][256]
+  int slabs, slab_cols;
 };
 struct NsArgs {
   NsMat t[NS_MAX_MATS];
@@ -227,10 +229,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const char* base) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0xffffffff, 0x00020000);
 }
 
-// workgroups that share a K range of kt K-tiles when `most` are offered: at least 8 each
+// Workgroups that share a K range of kt K-tiles when `most` are offered. Parts go through memory
+// and are waited for, 8 us a product at 1024 x 1024: a split is made where it takes 40 K-tiles or
+// more (0.2 us each) out of a workgroup's way, in parts of 16 or more. Whole call, split as here /
+// never / as often as offered: 512 x 512 139 / 139 / 158 us, 1024 x 1024 203 / 203 / 257, 2048 x
+// 2048 773 / 826 / 795, 300 x 8000 227 / 389 / 227, 8192 x 4096 6.66 / 7.42 / 6.66 ms.
 __host__ __device__ __forceinline__ int split_count(int kt, int most) {
-  const int fit = kt / 8;
-  return fit < 1 ? 1 : fit < most ? fit : most;
+  int s = kt / 16;
+  s = s < most ? s : most;
+  return s > 1 && kt - kt / s >= 40 ? s : 1;
 }
 
 // byte offset of 16-byte piece kc of a row inside an operand tile (rows of 128 bytes)
@@ -582,11 +589,16 @@ __global__ __launch_bounds__(T == 64 ? 512 : 256, T == 64 ? 4 : 2) void ns_produ
   ns_product_body<E, T, TO, MUON, T == 64>(args, step, ca, cb, cc, mo);
 }
 
+#include "newton_schulz_thin.h"
+
 // ---- host ------------------------------------------------------------------------------------
 long up(long v, long to) { return (v + to - 1) / to * to; }
 
+bool is_thin(long rows, long cols) { return (rows < cols ? rows : cols) <= THIN_M; }
+
 struct NsSizes {
   long m, n, km, kn, parts;
+  long slabs, slab_cols;          // thin matrices
   long x, xt, sq;                 // bytes of one image
   long total;
 };
@@ -594,6 +606,13 @@ NsSizes sizes_of(long rows, long cols) {
   NsSizes s;
   s.m = rows < cols ? rows : cols;
   s.n = rows < cols ? cols : rows;
+  if (is_thin(rows, cols)) {
+    s.slabs = thin_slabs(s.n);
+    s.slab_cols = up((s.n + s.slabs - 1) / s.slabs, 16);
+    s.total = up(s.slabs * THIN_GRAM * 8, 256);
+    return s;
+  }
+  s.slabs = s.slab_cols = 0;
   s.km = up(s.m, 32);
   s.kn = up(s.n, 32);
   const long want = (rows * cols + 4095) / 4096;
@@ -628,11 +647,6 @@ bool coefficients_fit(int steps, const float* coef) {
     r = top * (1.0 + 1e-3);              // between grid points, and for rounding
   }
   return true;
-}
-
-template <typename KernelT>
-void allow_lds(KernelT kernel, int lds) {
-  (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
 }
 
 // Which tiles of a product are split along K: those behind the last full round of the chip, as
@@ -694,14 +708,25 @@ int launch_steps(const NsArgs& args, int steps, const float* coef, const NsMuon&
 // tile size of a call: 128 once that many tiles give the chip's 256 CUs two workgroups each
 int tile_of(long tiles128) { return tiles128 >= NS_SLOTS ? 128 : 64; }
 
+// (thin matrices have no tiles)
+long tiles128_of(long rows, long cols) {
+  return is_thin(rows, cols) ? 0 : ((rows + 127) / 128) * ((cols + 127) / 128);
+}
+
 // head of the workspace: arrival counts, then the partial tiles of one split product
 constexpr long NS_HEAD = 4L * NS_SLOTS;
 long shared_bytes(int tile) { return NS_HEAD + 4L * NS_SLOTS * tile * tile; }
 
 template <typename E, bool MUON>
-int launch(const NsArgs& args, const NsArgs& parts, const NsArgs& split, int tile, int steps,
-           const float* coef, float eps, const NsMuon& mo, hipStream_t stream) {
+int launch(const NsArgs& args, const NsArgs& parts, const NsArgs& split, const NsArgs& thin,
+           int tile, int steps, const float* coef, float eps, const NsMuon& mo,
+           hipStream_t stream) {
+  if (thin.count) {
+    const int rc = launch_thin<E, MUON>(thin, steps, coef, eps, mo, stream);
+    if (rc != DTF_OK) return rc;
+  }
   const int n = args.count;
+  if (n == 0) return DTF_OK;
   hipLaunchKernelGGL((ns_norm_kernel<E, MUON>), dim3(parts.first[n]), dim3(256), 0, stream, parts,
                      mo);
   hipLaunchKernelGGL((ns_split_kernel<E, MUON>), dim3(split.first[n]), dim3(256), 0, stream, split,
@@ -721,26 +746,27 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     return DTF_ERR_BAD_ARG;
   if (count == 0) return DTF_OK;
   if (!coefficients_fit(steps, coef)) return DTF_ERR_UNSUPPORTED;
-  NsArgs args = {};
-  args.count = count;
+  // thin matrices have kernels of their own; the others share the tiled sequence
+  NsArgs args = {}, thin = {};
   char* at = (char*)workspace;
-  long used = 0, tiles128 = 0;
   if ((uintptr_t)at & 255) return DTF_ERR_BAD_ARG;
+  long used = 0, tiles128 = 0;
   for (int i = 0; i < count; ++i) {
     if (bad_shape(rows[i], cols[i])) return DTF_ERR_BAD_ARG;
-    tiles128 += ((rows[i] + 127L) / 128) * ((cols[i] + 127L) / 128);
+    tiles128 += tiles128_of(rows[i], cols[i]);
   }
   const int tile = tile_of(tiles128);
-  args.arrived = (int*)at;
-  args.partial = (float*)(at + NS_HEAD);
-  at += shared_bytes(tile);
-  used = shared_bytes(tile);
-  NsArgs parts, split;
+  if (tiles128 > 0) {
+    args.arrived = (int*)at;
+    args.partial = (float*)(at + NS_HEAD);
+    at += shared_bytes(tile);
+    used = shared_bytes(tile);
+  }
   for (int i = 0; i < count; ++i) {
-    if (!g[i] || !out[i] || (MUON && (!v[i])))
-      return DTF_ERR_BAD_ARG;
+    if (!g[i] || !out[i] || (MUON && (!v[i]))) return DTF_ERR_BAD_ARG;
     const NsSizes s = sizes_of(rows[i], cols[i]);
-    NsMat& t = args.t[i];
+    NsArgs& to = s.slabs ? thin : args;
+    NsMat& t = to.t[to.count++];
     t.g = g[i];
     t.out = out[i];
     t.v = MUON ? v[i] : nullptr;
@@ -749,11 +775,18 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     t.cols = cols[i];
     t.m = (int)s.m;
     t.n = (int)s.n;
+    used += s.total;
+    if (used > workspace_bytes) return DTF_ERR_BAD_ARG;
+    if (s.slabs) {
+      t.gram = (double*)at;
+      t.slabs = (int)s.slabs;
+      t.slab_cols = (int)s.slab_cols;
+      at += s.total;
+      continue;
+    }
     t.km = (int)s.km;
     t.kn = (int)s.kn;
     t.nparts = (int)s.parts;
-    used += s.total;
-    if (used > workspace_bytes) return DTF_ERR_BAD_ARG;
     t.parts = (double*)at;
     at += up(8 * s.parts, 256);
     t.x = at;
@@ -767,22 +800,24 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     t.b = at;
     at += s.sq;
   }
-  parts = split = args;
-  for (int i = 0; i < count; ++i) {
-    const long tiles = ((rows[i] + 63L) / 64) * ((cols[i] + 63L) / 64);
+  NsArgs parts = args, split = args;
+  for (int i = 0; i < args.count; ++i) {
+    const NsMat& t = args.t[i];
+    const long tiles = ((t.rows + 63L) / 64) * ((t.cols + 63L) / 64);
     if (split.first[i] + tiles > (1L << 30)) return DTF_ERR_UNSUPPORTED;
-    parts.first[i + 1] = parts.first[i] + args.t[i].nparts;
+    parts.first[i + 1] = parts.first[i] + t.nparts;
     split.first[i + 1] = split.first[i] + (int)tiles;
   }
   switch (type) {
-    case NS_F32: return launch<float, MUON>(args, parts, split, tile, steps, coef, eps, mo, stream);
+    case NS_F32:
+      return launch<float, MUON>(args, parts, split, thin, tile, steps, coef, eps, mo, stream);
     case NS_BF16:
       if constexpr (!MUON)
-        return launch<dtf_bf16, false>(args, parts, split, tile, steps, coef, eps, mo, stream);
+        return launch<dtf_bf16, false>(args, parts, split, thin, tile, steps, coef, eps, mo, stream);
       break;
     default:
       if constexpr (!MUON)
-        return launch<_Float16, false>(args, parts, split, tile, steps, coef, eps, mo, stream);
+        return launch<_Float16, false>(args, parts, split, thin, tile, steps, coef, eps, mo, stream);
       break;
   }
   return DTF_ERR_BAD_ARG;
@@ -796,10 +831,10 @@ DTF_API long dtf_newton_schulz_workspace(int count, const int* rows, const int* 
   long total = 256, tiles128 = 0;
   for (int i = 0; i < count; ++i) {
     if (bad_shape(rows[i], cols[i])) return 0;
-    tiles128 += ((rows[i] + 127L) / 128) * ((cols[i] + 127L) / 128);
+    tiles128 += tiles128_of(rows[i], cols[i]);
     total += sizes_of(rows[i], cols[i]).total;
   }
-  return total + shared_bytes(tile_of(tiles128));
+  return total + (tiles128 ? shared_bytes(tile_of(tiles128)) : 0);
 }
 
 // out[i] = orthogonalised g[i], both [rows[i], cols[i]] contiguous of `type` (0 fp32, 1 bf16,
