@@ -628,23 +628,31 @@ bool bad_shape(long rows, long cols) {
   return rows < 1 || cols < 1 || rows > (1L << 22) || cols > (1L << 22);
 }
 
-// Sizes of X, A and B over the steps, from the singular values' side: s in [0, r] -> p(s). The
-// stored fp16 images must hold every entry, and an entry is at most the largest singular value.
+// Sizes of X, A and B over the steps, from the singular values' side: s in [0, r] -> p(s) =
+// s q(s^2). The stored fp16 images must hold every entry, and an entry is at most the largest
+// singular value. The extremes of p and q lie at the ends and where a quadratic in t = s^2 has
+// its roots.
 bool coefficients_fit(int steps, const float* coef) {
   double r = 1.0 + 1e-6;
   for (int k = 0; k < steps; ++k) {
-    const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
-    double top = 0.0, b_top = 0.0;
-    constexpr int GRID = 4096;
-    for (int i = 0; i <= GRID; ++i) {
-      const double s = r * i / GRID, t = s * s;
+    const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2], end = r * r;
+    double p_top = 0.0, q_top = 0.0;
+    auto visit = [&](double t) {
+      if (!(t >= 0.0 && t <= end)) return;
       const double q = a + b * t + c * t * t;
-      if (!(q == q)) return false;
-      b_top = fmax(b_top, fabs(q));
-      top = fmax(top, fabs(s * q));
-    }
-    if (!(r * r <= AB_LIMIT) || !(b_top <= AB_LIMIT) || !(top <= X_LIMIT)) return false;
-    r = top * (1.0 + 1e-3);              // between grid points, and for rounding
+      p_top = fmax(p_top, fabs(sqrt(t) * q));
+      q_top = fmax(q_top, fabs(q));
+    };
+    if (!(fabs(a) + fabs(b) + fabs(c) < 1e30)) return false;
+    visit(0.0);
+    visit(end);
+    visit(-b / (2.0 * c));                       // q' = 0
+    const double root = sqrt(fmax(9.0 * b * b - 20.0 * a * c, 0.0));
+    visit((-3.0 * b + root) / (10.0 * c));       // p' = a + 3 b t + 5 c t^2 = 0
+    visit((-3.0 * b - root) / (10.0 * c));
+    visit(-a / (3.0 * b));                       // ... with c = 0
+    if (!(end <= AB_LIMIT) || !(q_top <= AB_LIMIT) || !(p_top <= X_LIMIT)) return false;
+    r = p_top * (1.0 + 1e-3);                    // (rounding of what is computed)
   }
   return true;
 }

@@ -143,7 +143,7 @@ __device__ __forceinline__ void thin_product(const double* P, const double* R, f
     const double* p = P + (16 * ti + (lane & 15)) * PITCH + (lane >> 4);
     const double* r = R + (16 * tj + (lane & 15)) * PITCH + (lane >> 4);
     f64x4 even = {0.0, 0.0, 0.0, 0.0}, odd = {0.0, 0.0, 0.0, 0.0};   // two chains: half the wait
-#pragma unroll 2
+#pragma unroll 4
     for (int k = 0; k < 16 * MT; k += 8) {
       even = mfma64(p[k], r[k], even);
       odd = mfma64(p[k + 4], r[k + 4], odd);
@@ -243,10 +243,12 @@ __device__ __forceinline__ void thin_apply(const NsMat& t, const NsMuon& mo, con
 #pragma unroll
     for (int b = 0; b < MT; ++b) acc[b] = f64x4{0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-    for (int k = 0; k < 4 * MT; ++k)
+    for (int k = 0; k < 4 * MT; ++k) {
 #pragma unroll
       for (int b = 0; b < MT; ++b)
         acc[b] = mfma64(Q[(16 * b + col) * PITCH + 4 * k + q], (double)u[k], acc[b]);
+      if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (all of Q in registers would spill)
+    }
 #pragma unroll
     for (int b = 0; b < MT; ++b)
 #pragma unroll
@@ -383,5 +385,6 @@ int launch_thin(const NsArgs& args, int steps, const float* coef, float eps, con
   // (blocks of 16 rows beyond a matrix's own hold zeros: they change no bit of its result)
   if (m <= 16) return launch_thin_of<E, MUON, 1>(args, st, eps, mo, stream);
   if (m <= 32) return launch_thin_of<E, MUON, 2>(args, st, eps, mo, stream);
+  if (m <= 48) return launch_thin_of<E, MUON, 3>(args, st, eps, mo, stream);
   return launch_thin_of<E, MUON, 4>(args, st, eps, mo, stream);
 }
