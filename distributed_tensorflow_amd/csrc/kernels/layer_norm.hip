@@ -7,9 +7,9 @@
 //             dgamma = sum over rows of dy h;  dbeta = sum over rows of dy
 //
 // Both directions move every element once and do about ten operations on it: they are bound by
-// memory. A row is held in registers by L lanes (16, 64, 256 or 1024: the fewest whose NV vectors
-// of 16 bytes cover it), so the second look at the row that the variance needs costs no second
-// read. Rows longer than 1024 lanes hold go through kernels that read them again.
+// memory. A row is held in registers by L lanes (a power of two from 4 to 1024, eight elements
+// each), so the second look at the row that the variance needs costs no second read. Rows longer
+// than 1024 lanes hold go through kernels that read them again.
 //
 // Everything between a load and a store is fp32. The variance is that of the differences from
 // the first mean, and what those differences sum to corrects both (the "corrected two-pass"
@@ -25,20 +25,26 @@ __device__ __forceinline__ float dpp_add(float v) {
   return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 
-// sum over groups of 16 lanes, in every lane of the group: quads, then the halves and the whole
-// of a 16-lane row by mirroring (a mirrored lane holds the other half's sum by then)
-__device__ __forceinline__ float sum16(float v) {
-  v = dpp_add<0xB1>(v);    // quad_perm [1, 0, 3, 2]
-  v = dpp_add<0x4E>(v);    // quad_perm [2, 3, 0, 1]
-  v = dpp_add<0x141>(v);   // row_half_mirror
-  return dpp_add<0x140>(v);   // row_mirror
+// sum over groups of 4, 8 or 16 lanes, in every lane of the group: quads, then the halves and the
+// whole of a 16-lane row by mirroring (a mirrored lane holds the other half's sum by then)
+template <int L>
+__device__ __forceinline__ float sum_row(float v) {
+  v = dpp_add<0xB1>(v);                  // quad_perm [1, 0, 3, 2]
+  v = dpp_add<0x4E>(v);                  // quad_perm [2, 3, 0, 1]
+  if (L >= 8) v = dpp_add<0x141>(v);     // row_half_mirror
+  if (L >= 16) v = dpp_add<0x140>(v);    // row_mirror
+  return v;
+}
+
+__device__ __forceinline__ float sum32(float v) {
+  v = sum_row<16>(v);
+  const unsigned u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 __device__ __forceinline__ float sum64(float v) {
-  v = sum16(v);
-  const unsigned u = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  v = sum32(v);
   const unsigned w = __float_as_uint(v);
   const auto s = __builtin_amdgcn_permlane32_swap(w, w, false, false);
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
@@ -49,9 +55,9 @@ __device__ __forceinline__ float sum64(float v) {
 // behind the barrier of the call in between, when every wave has read it).
 template <int L>
 __device__ __forceinline__ void group_sum2(float& a, float& b, float* red, int lane, int& turn) {
-  if (L == 16) {
-    a = sum16(a);
-    b = sum16(b);
+  if (L <= 32) {
+    a = L == 32 ? sum32(a) : sum_row<L>(a);
+    b = L == 32 ? sum32(b) : sum_row<L>(b);
     return;
   }
   a = sum64(a);
@@ -73,6 +79,8 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float* red, int l
     }
   }
 }
+
+constexpr int LANE_ELEMS = 8;
 
 template <typename T>
 constexpr int vec_of() {
@@ -105,7 +113,9 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layer_norm_kernel(
     if (beta) load_part<V>(beta, c, cols, bt[j]);
   }
   // (L >= 256: one row per workgroup, so the loop count is the same for every wave that meets at
-  // the barriers; smaller groups never leave their wave)
+  // the barriers; smaller groups never leave their wave. Requesting the next row before this one
+  // is worked on, as the backward kernel does, made the large cases 10-25 % slower: eight or more
+  // waves per SIMD cover the loads, and the registers cost some of them.)
   for (long row = blockIdx.x * (long)GROUPS + group; row < rows; row += (long)gridDim.x * GROUPS) {
     const T* xr = x + row * ldx;
     float v[NV][V];
@@ -120,14 +130,21 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layer_norm_kernel(
     const float m0 = s / (float)cols;     // (a constant row is its mean exactly)
     s = q = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      if ((j + 1) * L * V <= cols) {              // (the same for every lane)
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[j][k] -= m0;
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          v[j][k] = (lane + j * L) * V + k < cols ? v[j][k] - m0 : 0.f;
+      }
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float d = (lane + j * L) * V + k < cols ? v[j][k] - m0 : 0.f;
-        v[j][k] = d;
-        s += d;
-        q = __builtin_fmaf(d, d, q);
+        s += v[j][k];
+        q = __builtin_fmaf(v[j][k], v[j][k], q);
       }
+    }
     group_sum2<L>(s, q, my_red, lane, turn);
     const float fix = s * inv_n;
     const float var = __builtin_fmaf(-fix, fix, q * inv_n);
@@ -206,21 +223,24 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(
   }
 }
 
+constexpr int grad_block(int lanes) { return lanes > 512 ? lanes : 512; }
+
 // ---- backward -----------------------------------------------------------------------------
 // Every lane adds up dy h and dy of its columns over the rows it meets; the row groups of a
 // workgroup meet in LDS, the workgroups in `partial` [workgroups][2][cols] (summed in workgroup
 // order by the fold kernel: no atomics, the same bits every time). A single workgroup writes
 // dgamma and dbeta itself.
 template <typename T, typename P, int L, int NV>
-__global__ __launch_bounds__(L > 512 ? L : 512) void layer_norm_grad_kernel(
+__global__ __launch_bounds__(grad_block(L)) void layer_norm_grad_kernel(
     const T* __restrict__ dy, long ldd, const T* __restrict__ x, long ldx,
     const float* __restrict__ mean, const float* __restrict__ rstd, const P* __restrict__ gamma,
     T* __restrict__ dx, float* __restrict__ partial, P* __restrict__ dgamma,
     P* __restrict__ dbeta, long rows, int cols) {
   constexpr int V = vec_of<T>();
-  constexpr int BLOCK = L > 512 ? L : 512, GROUPS = BLOCK / L;
+  constexpr int BLOCK = grad_block(L), GROUPS = BLOCK / L;
   constexpr int RED = GROUPS * 4 * (L > 64 ? L / 64 : 1);
-  constexpr int FOLD = GROUPS > 1 ? BLOCK * 2 * V : 0;
+  // (rows of the fold are 64 / V words apart in banks: its readers walk along the columns)
+  constexpr int FPITCH = BLOCK + 64 / V, FOLD = GROUPS > 1 ? FPITCH * 2 * V : 0;
   __shared__ float sh[RED + FOLD];
   const int group = threadIdx.x / L, lane = threadIdx.x % L;
   float* my_red = sh + group * 4 * (L > 64 ? L / 64 : 1);
@@ -236,40 +256,52 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void layer_norm_grad_kernel(
     }
     if (gamma) load_part<V>(gamma, (lane + j * L) * V, cols, gm[j]);
   }
-  // every group runs the same number of turns (L = 256: two groups share the barriers); a group
-  // behind the last row works on zeros
-  for (long row0 = blockIdx.x * (long)GROUPS; row0 < rows; row0 += (long)gridDim.x * GROUPS) {
-    const long row = row0 + group;
+  // Every group runs the same number of turns (L = 256: the groups share the barriers); a group
+  // behind the last row works on zeros. The next row is requested before this one is
+  // worked on, except with 16 elements per lane, whose registers have no room for it.
+  constexpr bool AHEAD = L < 1024 || NV * V <= LANE_ELEMS;
+  Pack<T, V> nx[NV], nd[NV];
+  float nm = 0.f, nr = 0.f;
+  auto request = [&](long row) {
     const bool live = row < rows;
+    const long at = live ? row : 0;
     const int n = live ? cols : 0;
-    const T* xr = x + (live ? row : 0) * ldx;
-    const T* dr = dy + (live ? row : 0) * ldd;
-    const float m = live ? mean[row] : 0.f, r = live ? rstd[row] : 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      nx[j] = load_raw<V>(x + at * ldx, (lane + j * L) * V, n);
+      nd[j] = load_raw<V>(dy + at * ldd, (lane + j * L) * V, n);
+    }
+    nm = live ? mean[at] : 0.f;
+    nr = live ? rstd[at] : 0.f;
+  };
+  const long step = (long)gridDim.x * GROUPS;
+  if (AHEAD) request(blockIdx.x * (long)GROUPS + group);
+  for (long row0 = blockIdx.x * (long)GROUPS; row0 < rows; row0 += step) {
+    const long row = row0 + group;
+    if (!AHEAD) request(row);
+    const float m = nm, r = nr;
     float h[NV][V], g[NV][V];
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (lane + j * L) * V;
-      load_part<V>(xr, c, n, h[j]);
-      load_part<V>(dr, c, n, g[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
+      unpack(nx[j], h[j]);
+      unpack(nd[j], g[j]);
+      // (behind the row's end dy is zero, and so is everything added up here)
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float d = g[j][k];
-        const float hh = (lane + j * L) * V + k < n ? (h[j][k] - m) * r : 0.f;
+        const float d = g[j][k], hh = (h[j][k] - m) * r, gg = d * gm[j][k];
         ab[j][k] += d;
         ag[j][k] = __builtin_fmaf(d, hh, ag[j][k]);
-        const float gg = d * gm[j][k];
-        h[j][k] = hh;
-        g[j][k] = gg;
         s += gg;
         q = __builtin_fmaf(gg, hh, q);
+        h[j][k] = hh;
+        g[j][k] = gg;
       }
+    }
+    if (AHEAD) request(row + step);
     group_sum2<L>(s, q, my_red, lane, turn);
     const float sn = s * inv_n, qn = q * inv_n;
-    if (live) {
+    if (row < rows) {
       T* o = dx + row * (long)cols;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -302,20 +334,21 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void layer_norm_grad_kernel(
     if (j) __syncthreads();
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      fold[k * BLOCK + threadIdx.x] = ag[j][k];
-      fold[(V + k) * BLOCK + threadIdx.x] = ab[j][k];
+      fold[k * FPITCH + threadIdx.x] = ag[j][k];
+      fold[(V + k) * FPITCH + threadIdx.x] = ab[j][k];
     }
     __syncthreads();
     for (int t = threadIdx.x; t < 2 * V * L; t += BLOCK) {
-      const int k = t / L, l = t % L;
-      const int c = (l + j * L) * V + k % V;
+      const bool second = t >= V * L;
+      const int u = second ? t - V * L : t, l = u / V, k = (second ? V : 0) + u % V;
+      const int c = j * L * V + u;
       if (c >= cols) continue;
       float a = 0.f;
 #pragma unroll 8
-      for (int g2 = 0; g2 < GROUPS; ++g2) a += fold[k * BLOCK + g2 * L + l];
+      for (int g2 = 0; g2 < GROUPS; ++g2) a += fold[k * FPITCH + g2 * L + l];
       if (partial)
-        pg[(k < V ? 0 : cols) + c] = a;
-      else if (k < V) {
+        pg[(second ? cols : 0) + c] = a;
+      else if (!second) {
         if (dgamma) dgamma[c] = from_f32<P>(a);
       } else if (dbeta) {
         dbeta[c] = from_f32<P>(a);
@@ -387,81 +420,65 @@ __global__ __launch_bounds__(256) void layer_norm_grad_cols_kernel(
   p[cols + c] = b;
 }
 
-// partial [parts][2 cols] -> dgamma, dbeta: 64 columns per workgroup, 16 threads per column each
-// summing every 16th part, then a fixed tree over the 16
+// partial [parts][2 cols] -> dgamma, dbeta: 32 columns per workgroup, 32 threads per column each
+// summing every 32nd part, then the 32 in the lanes of a wave
 template <typename P>
 __global__ __launch_bounds__(1024) void layer_norm_fold_kernel(const float* __restrict__ partial,
                                                                int parts, P* __restrict__ dgamma,
                                                                P* __restrict__ dbeta, int cols) {
-  __shared__ float sh[16][64];
-  const int lx = threadIdx.x & 63, ly = threadIdx.x >> 6;
-  const long c = blockIdx.x * 64L + lx;
+  __shared__ float sh[32][33];
+  const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
+  const long c = blockIdx.x * 32L + lx;
   float a = 0.f;
   if (c < 2L * cols) {
 #pragma unroll 8
-    for (int p = ly; p < parts; p += 16) a += partial[p * 2L * cols + c];
+    for (int p = ly; p < parts; p += 32) a += partial[p * 2L * cols + c];
   }
-  sh[ly][lx] = a;
+  sh[lx][ly] = a;
   __syncthreads();
-  if (ly == 0 && c < 2L * cols) {
-    a = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) a += sh[k][lx];
-    if (c < cols) {
-      if (dgamma) dgamma[c] = from_f32<P>(a);
+  a = sum32(sh[ly][lx]);
+  const long d = blockIdx.x * 32L + ly;
+  if (lx == 0 && d < 2L * cols) {
+    if (d < cols) {
+      if (dgamma) dgamma[d] = from_f32<P>(a);
     } else if (dbeta) {
-      dbeta[c - cols] = from_f32<P>(a);
+      dbeta[d - cols] = from_f32<P>(a);
     }
   }
 }
 
 // ---- launch -------------------------------------------------------------------------------
-// (lanes, vectors per lane) for a row of `vecs` vectors of 16 bytes; lanes 0: the long-row
-// kernels. The backward kernel keeps five values per element in registers (x, dy, gamma and the
-// two column sums): 16 elements per lane are what fits without spilling; the forward kernel
-// keeps three and takes 32, except on 1024 lanes, where the register file leaves half as many.
+// (lanes, vectors per lane) for a row: eight elements per lane, 16 on 1024 lanes for the longest
+// rows; lanes 0: the long-row kernels. The backward kernel keeps seven values per element (x, dy,
+// gamma, the two column sums, and the next row's x and dy): with 16 elements per lane its 144
+// registers left one workgroup on a CU, and 16384 x 4096 bf16 took 136 us instead of 96.
 struct Plan {
   int lanes, nv;
 };
-Plan plan_of(long vecs, int v, bool grad) {
-  if (vecs <= 16) return {16, 1};
-  if (vecs <= 32) return {16, 2};
-  if (vecs <= 64) return {64, 1};
-  if (vecs <= 128) return {64, 2};
-  const bool four = !grad || v == 4;       // four vectors per lane fit
-  if (vecs <= 256) return four ? Plan{64, 4} : Plan{256, 1};
-  if (vecs <= 512) return {256, 2};
-  if (vecs <= 1024) return four ? Plan{256, 4} : Plan{1024, 1};
-  if (vecs <= 2048) return {1024, 2};
-  if (vecs <= 4096 && v == 4) return {1024, 4};
+Plan plan_of(long cols, int v) {
+  int lanes = 4;
+  while (lanes < 1024 && (long)lanes * LANE_ELEMS < cols) lanes *= 2;
+  if ((long)lanes * LANE_ELEMS >= cols) return {lanes, LANE_ELEMS / v};
+  if (lanes * 16L >= cols) return {lanes, 16 / v};
   return {0, 0};
 }
 
-// CALL(lanes, vectors per lane) of the plan; combinations no plan names are not compiled
-#define LN_FOR_PLAN(PLAN, GRAD, CALL)                                               \
-  switch ((PLAN).lanes * 8 + (PLAN).nv) {                                           \
-    case 16 * 8 + 1: CALL(16, 1); break;                                            \
-    case 16 * 8 + 2: CALL(16, 2); break;                                            \
-    case 64 * 8 + 1: CALL(64, 1); break;                                            \
-    case 64 * 8 + 2: CALL(64, 2); break;                                            \
-    case 256 * 8 + 2: CALL(256, 2); break;                                          \
-    case 1024 * 8 + 2: CALL(1024, 2); break;                                        \
-    case 64 * 8 + 4:                                                                \
-      if constexpr (!GRAD || V == 4) CALL(64, 4);                                   \
-      break;                                                                        \
-    case 256 * 8 + 4:                                                               \
-      if constexpr (!GRAD || V == 4) CALL(256, 4);                                  \
-      break;                                                                        \
-    case 256 * 8 + 1:                                                               \
-      if constexpr (GRAD && V == 8) CALL(256, 1);                                   \
-      break;                                                                        \
-    case 1024 * 8 + 1:                                                              \
-      if constexpr (GRAD && V == 8) CALL(1024, 1);                                  \
-      break;                                                                        \
-    case 1024 * 8 + 4:                                                              \
-      if constexpr (V == 4) CALL(1024, 4);                                          \
-      break;                                                                        \
-    default: break;                                                                 \
+// CALL(lanes, vectors per lane) of the plan
+#define LN_FOR_PLAN(PLAN, CALL)                                \
+  if ((PLAN).nv * V > LANE_ELEMS) {                                    \
+    CALL(1024, 16 / V);                                        \
+  } else {                                                     \
+    switch ((PLAN).lanes) {                                    \
+      case 4: CALL(4, LANE_ELEMS / V); break;                           \
+      case 8: CALL(8, LANE_ELEMS / V); break;                           \
+      case 16: CALL(16, LANE_ELEMS / V); break;                         \
+      case 32: CALL(32, LANE_ELEMS / V); break;                         \
+      case 64: CALL(64, LANE_ELEMS / V); break;                         \
+      case 128: CALL(128, LANE_ELEMS / V); break;                       \
+      case 256: CALL(256, LANE_ELEMS / V); break;                       \
+      case 512: CALL(512, LANE_ELEMS / V); break;                       \
+      default: CALL(1024, LANE_ELEMS / V); break;                       \
+    }                                                          \
   }
 
 long min_l(long a, long b) { return a < b ? a : b; }
@@ -470,7 +487,7 @@ template <typename T, typename P>
 int forward(const void* x, long ldx, const void* gamma, const void* beta, void* y, float* mean,
             float* rstd, long rows, long cols, float eps, hipStream_t stream) {
   constexpr int V = vec_of<T>();
-  const Plan p = plan_of((cols + V - 1) / V, V, false);
+  const Plan p = plan_of(cols, V);
   if (p.lanes == 0) {
     hipLaunchKernelGGL((layer_norm_long_kernel<T, P>), dim3((unsigned)min_l(rows, 512)),
                        dim3(1024), 0, stream, (const T*)x, ldx, (const P*)gamma, (const P*)beta,
@@ -482,20 +499,27 @@ int forward(const void* x, long ldx, const void* gamma, const void* beta, void* 
 #define LN_CALL(L_, NV_)                                                                     \
   hipLaunchKernelGGL((layer_norm_kernel<T, P, L_, NV_>), grid, block, 0, stream, (const T*)x, \
                      ldx, (const P*)gamma, (const P*)beta, (T*)y, mean, rstd, rows, (int)cols, eps)
-    LN_FOR_PLAN(p, false, LN_CALL)
+    LN_FOR_PLAN(p, LN_CALL)
 #undef LN_CALL
   }
   DTF_LAUNCH_CHECK();
   return DTF_OK;
 }
 
-// workgroups of the backward kernel: each leaves 2 cols partial sums behind
+// Workgroups of the backward kernel. Each turn of one takes about 1.4 us (a row per group, the
+// next one requested ahead), and each leaves 2 cols sums that are written and read again: 16 cols
+// bytes at 4 TB/s. The total is least at sqrt(turns * 350000 / cols) of them; up to four turns are
+// left to a single workgroup, which writes the result itself.
 int grad_parts(long rows, long cols, int v) {
-  const Plan p = plan_of((cols + v - 1) / v, v, true);
+  const Plan p = plan_of(cols, v);
   if (p.lanes == 0) return (int)min_l((rows + 15) / 16 > 0 ? (rows + 15) / 16 : 1, 64);
-  const int groups = p.lanes > 512 ? 1 : 512 / p.lanes;
-  const long want = (rows + groups - 1) / groups;
-  return (int)(want < 1 ? 1 : min_l(want, 512));
+  const int groups = grad_block(p.lanes) / p.lanes;
+  const long turns = (rows + groups - 1) / groups;
+  if (turns <= 4) return 1;
+  long best = (long)__builtin_sqrt((double)turns * 350000.0 / (double)cols);
+  best = min_l(best < 2 ? 2 : best, grad_block(p.lanes) > 512 ? 256 : 512);
+  const long each = (turns + best - 1) / best;
+  return (int)((turns + each - 1) / each);
 }
 
 template <typename T, typename P>
@@ -503,7 +527,7 @@ int backward(const void* dy, long ldd, const void* x, long ldx, const float* mea
              const float* rstd, const void* gamma, void* dx, float* partial, void* dgamma,
              void* dbeta, long rows, long cols, hipStream_t stream) {
   constexpr int V = vec_of<T>();
-  const Plan p = plan_of((cols + V - 1) / V, V, true);
+  const Plan p = plan_of(cols, V);
   const bool sums = dgamma || dbeta;
   const int parts = grad_parts(rows, cols, V);
   if (p.lanes == 0) {
@@ -518,7 +542,7 @@ int backward(const void* dy, long ldd, const void* x, long ldx, const float* mea
                          (const T*)dy, ldd, (const T*)x, ldx, mean, rstd, partial, rows,
                          (int)cols);
   } else {
-    const dim3 grid(parts), block(p.lanes > 512 ? p.lanes : 512);
+    const dim3 grid(parts), block(grad_block(p.lanes));
     const bool direct = parts == 1;
     float* part = sums && !direct ? partial : nullptr;
     P *dg = direct ? (P*)dgamma : nullptr, *db = direct ? (P*)dbeta : nullptr;
@@ -526,7 +550,7 @@ int backward(const void* dy, long ldd, const void* x, long ldx, const float* mea
   hipLaunchKernelGGL((layer_norm_grad_kernel<T, P, L_, NV_>), grid, block, 0, stream,         \
                      (const T*)dy, ldd, (const T*)x, ldx, mean, rstd, (const P*)gamma, (T*)dx, \
                      part, dg, db, rows, (int)cols)
-    LN_FOR_PLAN(p, true, LN_CALL)
+    LN_FOR_PLAN(p, LN_CALL)
 #undef LN_CALL
     if (direct) {
       DTF_LAUNCH_CHECK();
@@ -535,7 +559,7 @@ int backward(const void* dy, long ldd, const void* x, long ldx, const float* mea
   }
   DTF_LAUNCH_CHECK();
   if (sums) {
-    hipLaunchKernelGGL((layer_norm_fold_kernel<P>), dim3((unsigned)((2 * cols + 63) / 64)),
+    hipLaunchKernelGGL((layer_norm_fold_kernel<P>), dim3((unsigned)((2 * cols + 31) / 32)),
                        dim3(1024), 0, stream, partial, parts, (P*)dgamma, (P*)dbeta, (int)cols);
     DTF_LAUNCH_CHECK();
   }

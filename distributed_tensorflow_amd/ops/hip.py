@@ -1367,13 +1367,12 @@ def newton_schulz(g, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
     for start in range(0, len(work), _NS_GROUP):
         part = work[start:start + _NS_GROUP]
         n, t0 = len(part), part[0][0]
-        with _on_device(t0):
-            rows, cols, ws, base, size = _ns_workspace([t.shape for t, _ in part], t0.device, what)
-            g_arr = (ctypes.c_void_p * n)(*[t.data_ptr() for t, _ in part])
-            o_arr = (ctypes.c_void_p * n)(*[o.data_ptr() for _, o in part])
-            _ns_check(lib().dtf_newton_schulz(n, g_arr, o_arr, rows, cols, _NORM_TYPES[t0.dtype],
-                                              steps, coef, float(epsilon), base, size, _stream()),
-                      what)
+        rows, cols, ws, base, size = _ns_workspace([t.shape for t, _ in part], t0.device, what)
+        g_arr = (ctypes.c_void_p * n)(*[t.data_ptr() for t, _ in part])
+        o_arr = (ctypes.c_void_p * n)(*[o.data_ptr() for _, o in part])
+        _ns_check(_launch_on(t0.device, lib().dtf_newton_schulz, (
+            n, g_arr, o_arr, rows, cols, _NORM_TYPES[t0.dtype], steps, coef, float(epsilon), base,
+            size)), what)
     return result
 
 
@@ -1430,15 +1429,14 @@ def multi_muon(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     for start in range(0, len(work), _NS_GROUP):
         part = work[start:start + _NS_GROUP]
         n, w0 = len(part), part[0][0]
-        with _on_device(w0):
-            rows, cols, ws, base, size = _ns_workspace([w.shape for w, _, _, _ in part],
-                                                       w0.device, what)
-            arrays = [(c.c_void_p * n)(*[t[k].data_ptr() for t in part]) for k in range(3)]
-            s_arr = (c.c_float * n)(*[t[3] for t in part])
-            _ns_check(lib().dtf_multi_muon_f32(
-                n, arrays[0], arrays[1], arrays[2], s_arr, rows, cols, steps, coef,
-                float(epsilon), float(lr), _ptr(lr_dev), float(momentum), int(bool(nesterov)),
-                float(weight_decay), base, size, _stream()), what)
+        rows, cols, ws, base, size = _ns_workspace([w.shape for w, _, _, _ in part], w0.device,
+                                                   what)
+        arrays = [(c.c_void_p * n)(*[t[k].data_ptr() for t in part]) for k in range(3)]
+        s_arr = (c.c_float * n)(*[t[3] for t in part])
+        _ns_check(_launch_on(w0.device, lib().dtf_multi_muon_f32, (
+            n, arrays[0], arrays[1], arrays[2], s_arr, rows, cols, steps, coef, float(epsilon),
+            float(lr), _ptr(lr_dev), float(momentum), int(bool(nesterov)), float(weight_decay),
+            base, size)), what)
 
 
 def affine_scalars(scalars: Sequence[torch.Tensor], factors: Sequence[float],
@@ -2116,26 +2114,37 @@ def log_softmax_grad(y: torch.Tensor, dy: torch.Tensor) -> torch.Tensor:
 _NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _on_device(t: torch.Tensor):
-    """Context in which launches go to ``t``'s device (nothing to do when it is the current one)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch_on(device: torch.device, fn, args) -> int:
+    """``fn(*args, stream)`` on ``device``'s current stream, with ``device`` current meanwhile."""
+    # (building torch's Stream object takes 2.7 us of a call's 10: the raw handle is enough)
+    index = device.index
+    if index == torch.cuda.current_device():
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _norm_rows(t: torch.Tensor, what: str) -> torch.Tensor:
     """``t`` as a matrix of its last dimension's rows: contiguous rows at any pitch are taken as
     they lie, anything else is copied."""
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise HipKernelError("%s: expected a GPU tensor" % what)
     if t.dtype not in _NORM_TYPES:
         raise HipKernelError("%s: expected fp32, bf16 or fp16, got %s" % (what, t.dtype))
-    if t.dim() == 0 or t.shape[-1] == 0:
+    shape = t.shape
+    if not shape or shape[-1] == 0:
         raise HipKernelError("%s: needs a last dimension of at least one element, got shape %s"
-                             % (what, tuple(t.shape)))
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+                             % (what, tuple(shape)))
+    if len(shape) != 2:
+        t = t.reshape(-1, shape[-1])
+    if t.is_contiguous():
+        return t
+    rows, cols = t.shape
+    if (t.stride(1) == 1 or cols == 1) and (rows <= 1 or t.stride(0) >= cols):
         return t
     return t.contiguous()
 
@@ -2145,7 +2154,7 @@ def _norm_param(p: Optional[torch.Tensor], x: torch.Tensor, what: str) -> Option
         return None
     if not isinstance(p, torch.Tensor) or p.device != x.device:
         raise HipKernelError("%s: expected a tensor on the input's GPU" % what)
-    if p.dtype != x.dtype and p.dtype != torch.float32:
+    if p.dtype != torch.float32 and p.dtype != x.dtype:
         raise HipKernelError("%s: expected fp32 or the input's %s, got %s"
                              % (what, x.dtype, p.dtype))
     if p.numel() != x.shape[-1]:
@@ -2169,19 +2178,19 @@ def layer_norm(x: torch.Tensor, gamma: Optional[torch.Tensor] = None,
         raise HipKernelError("layer_norm: epsilon must not be negative, got %r" % (epsilon,))
     p = gamma if gamma is not None else beta
     rows, cols = x2.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if want_stats else None
+    device, dtype = x.device, x.dtype
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=dtype,
+                                                                   device=device)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=device).unbind(0)
     if rows:
-        base = stats.data_ptr() if want_stats else 0
-        with _on_device(x):
-            _check(lib().dtf_layer_norm(
-                x2.data_ptr(), x2.stride(0), _NORM_TYPES[x.dtype], _ptr(gamma), _ptr(beta),
-                _NORM_TYPES[p.dtype if p is not None else torch.float32], y.data_ptr(),
-                base or None, base + 4 * rows if base else None, rows, cols, float(epsilon),
-                _stream()), "layer_norm")
+        _check(_launch_on(device, lib().dtf_layer_norm, (
+            x2.data_ptr(), x2.stride(0), _NORM_TYPES[dtype], _ptr(gamma), _ptr(beta),
+            0 if p is None else _NORM_TYPES[p.dtype], y.data_ptr(), _ptr(mean), _ptr(rstd), rows,
+            cols, float(epsilon))), "layer_norm")
     if not want_stats:
         return y
-    mean, rstd = stats.unbind(0)
     if x.dim() != 2:
         mean, rstd = mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
     return y, mean, rstd
@@ -2212,29 +2221,30 @@ def layer_norm_grad(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
     if p_dtype != x.dtype and p_dtype != torch.float32:
         raise HipKernelError("layer_norm_grad: parameter gradients are fp32 or the input's %s"
                              % x.dtype)
-    kind = _NORM_TYPES[x.dtype]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    device, kind = x.device, _NORM_TYPES[x.dtype]
+    dx = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype,
+                                                                    device=device)
     sums = []
     for want, out in ((want_gamma, dgamma_out), (want_beta, dbeta_out)):
         if not want:
             sums.append(None)
         elif out is None:
-            sums.append(torch.empty((cols,), dtype=p_dtype, device=x.device))
-        elif p_dtype != torch.float32 or out.device != x.device:
+            sums.append(torch.empty((cols,), dtype=p_dtype, device=device))
+        elif p_dtype != torch.float32 or out.device != device:
             raise HipKernelError("layer_norm_grad: bad out tensor")
         else:
-            sums.append(_out_vec(out, cols, x.device, "layer_norm_grad"))
+            sums.append(_out_vec(out, cols, device, "layer_norm_grad"))
     dgamma, dbeta = sums
     L = lib()
     ws = None
     if want_gamma or want_beta:
-        ws = torch.empty((L.dtf_layer_norm_grad_workspace(rows, cols, kind),),
-                         dtype=torch.float32, device=x.device)
-    with _on_device(x):
-        _check(L.dtf_layer_norm_grad(
-            dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), kind, mean.data_ptr(),
-            rstd.data_ptr(), _ptr(gamma), _NORM_TYPES[p_dtype], dx.data_ptr(), _ptr(ws),
-            _ptr(dgamma), _ptr(dbeta), rows, cols, _stream()), "layer_norm_grad")
+        words = L.dtf_layer_norm_grad_workspace(rows, cols, kind)
+        if words:
+            ws = torch.empty((words,), dtype=torch.float32, device=device)
+    _check(_launch_on(device, L.dtf_layer_norm_grad, (
+        dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), kind, mean.data_ptr(),
+        rstd.data_ptr(), _ptr(gamma), _NORM_TYPES[p_dtype], dx.data_ptr(), _ptr(ws), _ptr(dgamma),
+        _ptr(dbeta), rows, cols)), "layer_norm_grad")
     return dx, dgamma, dbeta
 
 

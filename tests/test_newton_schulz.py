@@ -94,13 +94,13 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
     ints = lambda *v: (ctypes.c_int * len(v))(*v)                       # noqa: E731
     ptrs = lambda *v: (ctypes.c_void_p * len(v))(*v)                    # noqa: E731
     coef = lambda *v: (ctypes.c_float * len(v))(*v)                     # noqa: E731
-    need = lib.dtf_newton_schulz_workspace(1, ints(64), ints(32))
-    assert need > 4 * (64 * 32 * 3 + 32 * 32 * 2)
+    need = lib.dtf_newton_schulz_workspace(1, ints(96), ints(80))
+    assert need > 4 * (96 * 80 * 3 + 80 * 80 * 2)
     for bad in ((0, 5), (5, 0), (-1, 5), (1 << 23, 5)):
         assert lib.dtf_newton_schulz_workspace(1, ints(bad[0]), ints(bad[1])) == 0
     assert lib.dtf_newton_schulz_workspace(17, ints(*[4] * 17), ints(*[4] * 17)) == 0
 
-    def call(count=1, g=4096, out=4096, rows=64, cols=32, type_=0, steps=1, c=COEF, eps=1e-7,
+    def call(count=1, g=4096, out=4096, rows=96, cols=80, type_=0, steps=1, c=COEF, eps=1e-7,
              ws=4096, size=need):
         return lib.dtf_newton_schulz(count, ptrs(g), ptrs(out), ints(rows), ints(cols), type_,
                                      steps, coef(*c), eps, ws, size, None)
@@ -112,8 +112,8 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
     for c in ((9.0, 0.0, 0.0), (float("nan"), 0.0, 0.0), (20.0, -40.0, 20.0)):
         assert call(c=c) == -2, c
     one = ctypes.c_float * 1
-    assert lib.dtf_multi_muon_f32(1, ptrs(4096), ptrs(4096), ptrs(None), one(1.0), ints(64),
-                                  ints(32), 1, coef(*COEF), 1e-7, 0.1, None, 0.9, 1, 0.0, 4096,
+    assert lib.dtf_multi_muon_f32(1, ptrs(4096), ptrs(4096), ptrs(None), one(1.0), ints(96),
+                                  ints(80), 1, coef(*COEF), 1e-7, 0.1, None, 0.9, 1, 0.0, 4096,
                                   need, None) == -1
     for call in (lambda: hip.newton_schulz(torch.zeros(3, 4)),
                  lambda: hip.newton_schulz([torch.zeros(3, 4)]),
