@@ -35,7 +35,7 @@ namespace {
 constexpr int NS_CHAIN = 4;            // K-tiles an accumulator runs through before it is emptied
 constexpr int NS_MAX_MATS = 16;
 constexpr int NS_MAX_STEPS = 32;
-constexpr int NS_SLOTS = 512;          // workgroups of a product that run at once: two per CU
+constexpr int NS_SLOTS = 512;          // workgroups of a product that run at once, at most
 constexpr int NS_MAX_PARTS = 1024;     // workgroups that share a matrix's sum of squares
 constexpr float X_SCALE = 16384.f, AB_SCALE = 4096.f;
 constexpr double X_LIMIT = 3.5, AB_LIMIT = 15.0;   // times the scales: below fp16's 65504
@@ -117,6 +117,9 @@ __device__ __forceinline__ void store_split8(char* chunk_hi, const unsigned* p) 
 // byte offset of element c in a split row (its hi half; the lo half is 64 bytes further)
 __device__ __forceinline__ long split_off(int c) { return (long)(c >> 5) * 128 + (c & 31) * 2; }
 
+// (padding the pitch off the powers of two made the large products 1 to 9 % slower)
+__host__ __device__ __forceinline__ long pitch_of(int k) { return 4L * k; }
+
 // ---- momentum and sum of squares -------------------------------------------------------------
 // Squares are summed in 64 bits: gradients of 1e-20 or 1e+25 have squares fp32 does not hold.
 template <typename E, bool MUON>
@@ -196,8 +199,8 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, float eps, N
   const bool tall = t.rows > t.cols;
   char* direct = tall ? t.xt0 : t.x;               // rows of `cols` elements
   char* turned = tall ? t.x : t.xt0;               // rows of `rows` elements
-  const long direct_pitch = 4L * (tall ? t.km : t.kn);
-  const long turned_pitch = 4L * (tall ? t.kn : t.km);
+  const long direct_pitch = pitch_of(tall ? t.km : t.kn);
+  const long turned_pitch = pitch_of(tall ? t.kn : t.km);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int rl = (threadIdx.x >> 3) + 32 * h, r = r0 + rl;
@@ -231,9 +234,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const char* base) {
 
 // Workgroups that share a K range of kt K-tiles when `most` are offered. Parts go through memory
 // and are waited for, 8 us a product at 1024 x 1024: a split is made where it takes 40 K-tiles or
-// more (0.2 us each) out of a workgroup's way, in parts of 16 or more. Whole call, split as here /
-// never / as often as offered: 512 x 512 139 / 139 / 158 us, 1024 x 1024 203 / 203 / 257, 2048 x
-// 2048 773 / 826 / 795, 300 x 8000 227 / 389 / 227, 8192 x 4096 6.66 / 7.42 / 6.66 ms.
+// more (0.2 us each on 64 x 64 tiles) out of a workgroup's way, in parts of 16 or more. Whole
+// call, split as here / never / as often as offered: 1024 x 1024 195 / 195 / 257 us, 2048 x 2048
+// 748 / 797 / 874, 300 x 8000 213 / 378 / 213, 1024 x 4096 371 / 403 / 398, 1024 x 8192 617 / 700 /
+// 850, 8192 x 4096 6.30 / 7.34 / 6.37 ms.
 __host__ __device__ __forceinline__ int split_count(int kt, int most) {
   int s = kt / 16;
   s = s < most ? s : most;
@@ -245,147 +249,320 @@ __device__ __forceinline__ int piece_off(int row, int kc) {
   return row * 128 + ((kc ^ ((row >> 1) & 7)) << 4);
 }
 
-// One T x T tile of P Q^T, P [M][K] and Q [N][K] in split rows, by four waves of T/2 x T/2.
-// TO_A / TO_B: symmetric results (M = N, tiles on and below the diagonal), written to both
-// places; TO_X: written in both orders; TO_OUT: the caller's type.
-//
-// K loop. WS: four more waves issue the LDS-DMA requests, NB - 1 K-tiles ahead into NB buffers,
-// so that the multiplying waves never wait at the address unit. Otherwise two buffers, and a
-// second workgroup on the CU covers the waits.
+// One BM x BN tile of P Q^T, P [M][K] and Q [N][K] in split rows. TO_A / TO_B: symmetric results
+// (M = N, tiles on and below the diagonal), written to both places; TO_X: written in both orders;
+// TO_OUT: the caller's type.
 //
 // Accumulation. The matrix instruction adds its 32 products to the accumulator in steps of its
 // own; a long chain of them loses more than fp32 sums of rounded products do (1024 x 1024: the
 // result was off by 4.7e-6, an fp32 computation by 3.1e-6). Every NS_CHAIN K-tiles the
-// accumulators are added to a second set and start again from zero.
+// accumulators are added to a second set and start again from zero (2.2e-6; no time).
 //
 // Splits. A tile whose K range is shared leaves fp32 partial tiles in memory; the workgroup that
 // arrives last adds all of them in split order, whoever it is, so the bits do not depend on the
 // order of arrival.
-template <typename E, int T, int TO, bool MUON, bool WS>
-__device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, float ca, float cb,
-                                                float cc, const NsMuon& mo) {
-  constexpr int NI = T / 32;                    // 16 x 16 tiles per wave and direction
-  constexpr int WT = T / 2;
-  constexpr int OP_BYTES = T * 128, BUF_BYTES = 2 * OP_BYTES;
-  constexpr int NB = WS ? 4 : 2;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wave = wave8 & 3;
-  const bool producer = WS && wave8 >= 4;
-  const int wr = wave >> 1, wc = wave & 1;
-  int id, split = 0, splits = 1;
+struct NsTile {
+  const char *P, *Q;
+  int M, N, K;
+  int m0, n0;
+  int kt0, nkt;              // this workgroup's K-tiles
+  int mat, shared, split, splits;
+};
+
+// this workgroup's tile; false: nothing to do
+template <int BM, int BN, int TO>
+__device__ __forceinline__ bool ns_locate(const NsArgs& args, int step, NsTile& w) {
+  int id;
+  w.split = 0;
+  w.splits = 1;
   if ((int)blockIdx.x < args.unsplit) {
     id = dtf_xcd_remap(blockIdx.x, args.unsplit);
   } else {
-    const int r = blockIdx.x - args.unsplit;
-    splits = args.splits;
-    id = args.unsplit + r / splits;
-    split = r % splits;
+    // an XCD takes neighbouring tiles of one K range, whose rows its L2 holds (the parts of a tile
+    // side by side instead, so on several XCDs: 1024 x 8192 726 us, here 617)
+    const int rest = args.first[args.count] - args.unsplit;
+    w.splits = args.splits;
+    const int r = dtf_xcd_remap(blockIdx.x - args.unsplit, rest * w.splits);
+    id = args.unsplit + r % rest;
+    w.split = r / rest;
   }
-  const int shared_tile = id - args.unsplit;
-  const int mat = matrix_of(args, id);
-  const NsMat& t = args.t[mat];
-  const int tile = id - args.first[mat];
-
-  const bool tall = t.rows > t.cols;
-  const char *P, *Q;
-  int M, N, K;
+  w.shared = id - args.unsplit;
+  w.mat = matrix_of(args, id);
+  const NsMat& t = args.t[w.mat];
+  const int tile = id - args.first[w.mat];
   if (TO == TO_A) {
-    P = Q = t.x; M = N = t.m; K = t.kn;
+    w.P = w.Q = t.x; w.M = w.N = t.m; w.K = t.kn;
   } else if (TO == TO_B) {
-    P = Q = t.a; M = N = t.m; K = t.km;
+    w.P = w.Q = t.a; w.M = w.N = t.m; w.K = t.km;
   } else {
     const char* xt = (step & 1) ? t.xt1 : t.xt0;
-    K = t.km;
-    if (TO == TO_OUT && tall) {                 // X^T = X^T B: the result as the caller lays it
-      P = xt; Q = t.b; M = t.n; N = t.m;
+    w.K = t.km;
+    if (TO == TO_OUT && t.rows > t.cols) {      // X^T = X^T B: the result as the caller lays it
+      w.P = xt; w.Q = t.b; w.M = t.n; w.N = t.m;
     } else {
-      P = t.b; Q = xt; M = t.m; N = t.n;
+      w.P = t.b; w.Q = xt; w.M = t.m; w.N = t.n;
     }
   }
-  const int all_kt = K / 32;
-  if (splits > 1) {                             // (a matrix with a short K uses fewer)
-    splits = split_count(all_kt, splits);
-    if (split >= splits) return;
+  const int all_kt = w.K / 32;
+  if (w.splits > 1) {                           // (a matrix with a short K uses fewer)
+    w.splits = split_count(all_kt, w.splits);
+    if (w.split >= w.splits) return false;
   }
-  const int kt0 = (int)((long)all_kt * split / splits);
-  const int nkt = (int)((long)all_kt * (split + 1) / splits) - kt0;
+  w.kt0 = (int)((long)all_kt * w.split / w.splits);
+  w.nkt = (int)((long)all_kt * (w.split + 1) / w.splits) - w.kt0;
   int tm, tn;
   if (TO == TO_A || TO == TO_B) {
-    tm = (int)((__builtin_sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-    while ((tm + 1) * (tm + 2) / 2 <= tile) ++tm;
-    while (tm * (tm + 1) / 2 > tile) --tm;
-    tn = tile - tm * (tm + 1) / 2;
+    // row tm of the triangle has F (tm + 1) tiles: F tm (tm + 1) / 2 before it
+    constexpr int F = BM / BN;
+    tm = (int)((__builtin_sqrtf(8.f / F * tile + 1.f) - 1.f) * 0.5f);
+    while (F * (tm + 1) * (tm + 2) / 2 <= tile) ++tm;
+    while (F * tm * (tm + 1) / 2 > tile) --tm;
+    tn = tile - F * tm * (tm + 1) / 2;
   } else {
     constexpr int GROUP = 8;
-    const int tiles_m = (M + T - 1) / T, tiles_n = (N + T - 1) / T;
+    const int tiles_m = (w.M + BM - 1) / BM, tiles_n = (w.N + BN - 1) / BN;
     const int per_group = GROUP * tiles_n, grp = tile / per_group, first_m = grp * GROUP;
     const int gsize = tiles_m - first_m < GROUP ? tiles_m - first_m : GROUP;
     tm = first_m + tile % per_group % gsize;
     tn = tile % per_group / gsize;
   }
-  const int m0 = tm * T, n0 = tn * T;
-  const long pitch = 4L * K;
+  w.m0 = tm * BM;
+  w.n0 = tn * BN;
+  return true;
+}
 
-  unsigned voff_p[NI], voff_q[NI];
+// The parts of a shared tile. True in the workgroup that has all of them in `sum`. The XCDs' L2s
+// do not see each other's lines, so the parts go through memory: stores and loads of device scope
+// pass the L2 by, and a store is complete once it has arrived there. (A release fence instead
+// writes the whole L2 back, 0.4 us each and one after the other on an XCD: 29 us for a product at
+// 1024 x 1024 split three ways.) The first THREADS threads hold the tile.
+template <int NM, int NN, int THREADS>
+__device__ __forceinline__ bool ns_join(f32x4 (&sum)[NM][NN], const NsArgs& args, const NsTile& w) {
+  __shared__ int last;
+  constexpr int PAIRS = NM * NN * 2 * THREADS;  // 8-byte pairs in a partial tile
+  const bool holds = threadIdx.x < THREADS;
+  typedef unsigned long long pair_t;
+  pair_t* part = reinterpret_cast<pair_t*>(args.partial) + (long)w.shared * args.splits * PAIRS +
+                 threadIdx.x;
+  if (holds) {
+    pair_t* mine = part + (long)w.split * PAIRS;
 #pragma unroll
-  for (int j = 0; j < NI; ++j) {
-    const int row = (wave * NI + j) * 8 + (lane >> 3);
-    const int kc = (lane & 7) ^ ((row >> 1) & 7);
-    const int rp = m0 + row < M ? row : M - 1 - m0, rq = n0 + row < N ? row : N - 1 - n0;
-    voff_p[j] = (unsigned)rp * (unsigned)pitch + 16u * kc;
-    voff_q[j] = (unsigned)rq * (unsigned)pitch + 16u * kc;
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+      for (int j = 0; j < NN; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const pair_t v = (pair_t)__float_as_uint(sum[i][j][2 * h]) |
+                           (pair_t)__float_as_uint(sum[i][j][2 * h + 1]) << 32;
+          __hip_atomic_store(mine + ((i * NN + j) * 2 + h) * THREADS, v, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+        }
   }
-  const __amdgpu_buffer_rsrc_t p_rsrc = rows_rsrc(P + m0 * pitch);
-  const __amdgpu_buffer_rsrc_t q_rsrc = rows_rsrc(Q + n0 * pitch);
-  auto request = [&](int kt, char* buf) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's part has arrived ...
+  __syncthreads();                                   // ... and every wave's, before the count
+  if (threadIdx.x == 0) {
+    const int before = __hip_atomic_fetch_add(&args.arrived[w.shared], 1, __ATOMIC_RELAXED,
+                                              __HIP_MEMORY_SCOPE_AGENT);
+    last = before == w.splits - 1;
+    if (last)                                   // nobody else comes: ready for the next launch
+      __hip_atomic_store(&args.arrived[w.shared], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last || !holds) return false;
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int piece = wave * NI + j;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(p_rsrc, (lds_void*)(buf + piece * 1024), 16,
-                                               voff_p[j], kt * 128, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(q_rsrc, (lds_void*)(buf + OP_BYTES + piece * 1024),
-                                               16, voff_q[j], kt * 128, 0, 0);
+  for (int i = 0; i < NM; ++i)
+#pragma unroll
+    for (int j = 0; j < NN; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < w.splits; ++k) {
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      pair_t v[NN][2];
+#pragma unroll
+      for (int j = 0; j < NN; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          v[j][h] = __hip_atomic_load(part + ((i * NN + j) * 2 + h) * THREADS, __ATOMIC_RELAXED,
+                                      __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int j = 0; j < NN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          sum[i][j][r] += __uint_as_float((unsigned)(v[j][r >> 1] >> (32 * (r & 1))));
     }
-  };
+    part += PAIRS;
+  }
+  return true;
+}
 
+// Results of one wave: rows mw + 16 i + lane % 16, columns nw + 16 j + 4 (lane / 16) + 0..3.
+// `strip`: 16 NN rows of 36 dwords of LDS, this wave's own.
+template <typename E, int NM, int NN, int TO, bool MUON>
+__device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsMat& t,
+                                         const NsTile& w, int step, float ca, float cb, float cc,
+                                         const NsMuon& mo, int mw, int nw, unsigned* strip) {
+  const int lane = threadIdx.x & 63, frow = lane & 15, fq = lane >> 4;
+  const int mb = mw + frow, nb = nw + 4 * fq, M = w.M, N = w.N;
+  if (TO == TO_OUT) {
+    const float lr = MUON ? (mo.lr_dev ? mo.lr_dev[0] : mo.lr) : 0.f;
+    const float keep = 1.f - lr * mo.decay, take = lr * t.scale;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const int m = mb + 16 * i;
+      if (m >= M) continue;
+      E* row = (E*)t.out + (long)m * N;
+#pragma unroll
+      for (int j = 0; j < NN; ++j) {
+        const int n = nb + 16 * j;
+        if (n >= N) continue;
+        float v[4], old[4];
+        if (MUON) load_part<4>(row, n, N, old);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          v[r] = acc[i][j][r] * (1.f / (X_SCALE * AB_SCALE));
+          if (MUON) v[r] = __builtin_fmaf(-take, v[r], keep * old[r]);
+        }
+        store_part<4>(row, n, N, v);
+      }
+    }
+    return;
+  }
+  constexpr bool SYM = TO == TO_A || TO == TO_B;
+  // (squares of this wave's size: above the diagonal the mirror image writes)
+  const int row_block = mw / (16 * NM), col_block = nw / (16 * NN);
+  if (SYM && row_block < col_block) return;
+  char* direct = TO == TO_A ? t.a : TO == TO_B ? t.b : t.x;            // rows along M
+  char* turned = TO == TO_X ? ((step & 1) ? t.xt0 : t.xt1) : direct;   // rows along N
+  const long d_pitch = pitch_of(TO == TO_X ? t.kn : t.km), t_pitch = pitch_of(t.km);
+#pragma unroll
+  for (int h = 0; h < NM / 2; ++h) {
+    // packed (hi | lo << 16) results; zero behind the last row and column
+    unsigned pk[2][NN][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NN; ++j) {
+        const int m = mb + 16 * (2 * h + i), n = nb + 16 * j;
+        f32x4 v = acc[2 * h + i][j];
+        if (TO == TO_A) v *= AB_SCALE / (X_SCALE * X_SCALE);
+        if (TO == TO_X) v *= 1.f / AB_SCALE;
+        if (TO == TO_B) {
+          f16x4 ah = {0, 0, 0, 0}, al = {0, 0, 0, 0};
+          if (m < M && (n & ~31) < N) {
+            const char* src = t.a + m * t_pitch + split_off(n);
+            ah = *reinterpret_cast<const f16x4*>(src);
+            al = *reinterpret_cast<const f16x4*>(src + 64);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            v[r] = __builtin_fmaf(cc / AB_SCALE, v[r],
+                                  __builtin_fmaf(cb, (float)ah[r] + (float)al[r],
+                                                 m == n + r ? ca * AB_SCALE : 0.f));
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pk[i][j][r] = m < M && n + r < N ? split_pack(v[r]) : 0u;
+        if (m < M && (n & ~31) < N) {
+          char* dst = direct + m * d_pitch + split_off(n);
+          const unsigned* p = pk[i][j];
+          *reinterpret_cast<uint2*>(dst) = uint2{(p[0] & 0xffffu) | p[1] << 16,
+                                                 (p[2] & 0xffffu) | p[3] << 16};
+          *reinterpret_cast<uint2*>(dst + 64) = uint2{p[0] >> 16 | (p[1] & 0xffff0000u),
+                                                      p[2] >> 16 | (p[3] & 0xffff0000u)};
+        }
+      }
+    if (SYM && row_block == col_block) continue;   // a diagonal block is its own mirror image
+    // the other order through the strip: [16 NN of N][32 of M]
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          strip[(16 * j + 4 * fq + r) * 36 + 16 * i + frow] = pk[i][j][r];
+    __builtin_amdgcn_wave_barrier();
+    const int mc = mw + 32 * h;                    // first element of the chunk
+#pragma unroll
+    for (int q = 0; q < NN; ++q) {
+      const int nl = 16 * q + (lane >> 2), n = nw + nl;
+      unsigned p[8];
+      const u32x4* src = reinterpret_cast<const u32x4*>(strip + nl * 36 + (lane & 3) * 8);
+      *reinterpret_cast<u32x4*>(p) = src[0];
+      *reinterpret_cast<u32x4*>(p + 4) = src[1];
+      if (n < N && mc < M) store_split8(turned + n * t_pitch + split_off(mc + (lane & 3) * 8), p);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// 64 x 64 tiles: four multiplying waves and four that issue the LDS-DMA requests, three K-tiles
+// ahead into four buffers -- the multiplying waves never wait at the address unit. Two workgroups
+// per CU. (Four waves that do both: 1024 x 1024 302 us instead of 186.)
+template <typename E, int TO, bool MUON>
+__device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, float ca, float cb,
+                                              float cc, const NsMuon& mo) {
+  constexpr int T = 64, NI = 2, WT = 32, NB = 4;
+  constexpr int OP_BYTES = T * 128, BUF_BYTES = 2 * OP_BYTES;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave8 & 3;
+  const bool producer = wave8 >= 4;
+  const int wr = wave >> 1, wc = wave & 1;
+  NsTile w;
+  if (!ns_locate<T, T, TO>(args, step, w)) return;
+  const NsMat& t = args.t[w.mat];
   f32x4 sum[NI][NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
 #pragma unroll
     for (int j = 0; j < NI; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int frow = lane & 15, fq = lane >> 4;
-  if (WS && producer) {
+  if (producer) {
     constexpr int R = 2 * NI;                   // requests per wave and K-tile
-    for (int kt = 0; kt < NB - 1 && kt < nkt; ++kt) request(kt0 + kt, smem + kt * BUF_BYTES);
-    for (int kt = 0; kt < nkt; ++kt) {
+    const long pitch = pitch_of(w.K);
+    unsigned voff_p[NI], voff_q[NI];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int row = (wave * NI + j) * 8 + (lane >> 3);
+      const int kc = (lane & 7) ^ ((row >> 1) & 7);
+      const int rp = w.m0 + row < w.M ? row : w.M - 1 - w.m0;
+      const int rq = w.n0 + row < w.N ? row : w.N - 1 - w.n0;
+      voff_p[j] = (unsigned)rp * (unsigned)pitch + 16u * kc;
+      voff_q[j] = (unsigned)rq * (unsigned)pitch + 16u * kc;
+    }
+    const __amdgpu_buffer_rsrc_t p_rsrc = rows_rsrc(w.P + w.m0 * pitch);
+    const __amdgpu_buffer_rsrc_t q_rsrc = rows_rsrc(w.Q + w.n0 * pitch);
+    auto request = [&](int kt) {
+      char* buf = smem + kt % NB * BUF_BYTES;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int piece = wave * NI + j, at = (w.kt0 + kt) * 128;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(p_rsrc, (lds_void*)(buf + piece * 1024), 16,
+                                                 voff_p[j], at, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            q_rsrc, (lds_void*)(buf + OP_BYTES + piece * 1024), 16, voff_q[j], at, 0, 0);
+      }
+    };
+    for (int kt = 0; kt < NB - 1 && kt < w.nkt; ++kt) request(kt);
+    for (int kt = 0; kt < w.nkt; ++kt) {
       // own pieces of K-tile kt have landed; those of up to NB - 2 later ones stay in flight
-      if (nkt - 1 - kt >= 2)
+      if (w.nkt - 1 - kt >= 2)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * R) : "memory");
-      else if (nkt - 1 - kt == 1)
+      else if (w.nkt - 1 - kt == 1)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R) : "memory");
       else
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       asm volatile("s_barrier" ::: "memory");
       // behind the barrier the multiplying waves are done with the buffer of K-tile kt - 1
-      if (kt + NB - 1 < nkt) request(kt0 + kt + NB - 1, smem + (kt + NB - 1) % NB * BUF_BYTES);
+      if (kt + NB - 1 < w.nkt) request(kt + NB - 1);
     }
     asm volatile("s_barrier" ::: "memory");
-    if (splits == 1) return;
+    if (w.splits == 1) return;
   } else {
-    if (!WS) request(kt0, smem);
     f32x4 acc[NI][NI];
     // one K-tile; FIRST: the accumulators start from zero
     auto multiply = [&](int kt, auto first) {
       constexpr bool FIRST = decltype(first)::value;
       // K-tile kt has landed for every wave, and every wave is done with the buffer before it
-      if (WS) {
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (kt + 1 < nkt) request(kt0 + kt + 1, smem + ((kt + 1) & 1) * BUF_BYTES);
-      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       const char* cur = smem + kt % NB * BUF_BYTES;
       f16x8 ph[NI], pl[NI], qh[NI], ql[NI];
 #pragma unroll
@@ -407,9 +584,9 @@ __device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, fl
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph[i], acc[i][j], 0, 0, 0);
         }
     };
-    for (int base = 0; base < nkt; base += NS_CHAIN) {
+    for (int base = 0; base < w.nkt; base += NS_CHAIN) {
       multiply(base, yes());
-      const int end = base + NS_CHAIN < nkt ? base + NS_CHAIN : nkt;
+      const int end = base + NS_CHAIN < w.nkt ? base + NS_CHAIN : w.nkt;
       for (int kt = base + 1; kt < end; ++kt) multiply(kt, no());
 #pragma unroll
       for (int i = 0; i < NI; ++i)
@@ -419,174 +596,139 @@ __device__ __forceinline__ void ns_product_body(const NsArgs& args, int step, fl
     // the buffers become the epilogue's scratch
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
+  if (w.splits > 1 && !ns_join<NI, NI, 256>(sum, args, w)) return;
+  ns_store<E, NI, NI, TO, MUON>(sum, t, w, step, ca, cb, cc, mo, w.m0 + wr * WT, w.n0 + wc * WT,
+                                reinterpret_cast<unsigned*>(smem) + wave * (WT * 36));
+}
 
-  if (splits > 1) {
-    __shared__ int last;
-    constexpr int PAIRS = T * T / 2;            // 8-byte pairs in a partial tile
-    typedef unsigned long long pair_t;
-    pair_t* mine = reinterpret_cast<pair_t*>(args.partial) +
-                   ((long)shared_tile * args.splits + split) * PAIRS + (tid & 255);
-    // The XCDs' L2s do not see each other's lines, so the parts go through memory: stores and
-    // loads of device scope pass the L2 by, and a store is complete once it has arrived there.
-    // (A release fence instead writes the whole L2 back, 0.4 us each and one after the other on
-    // an XCD: 29 us for this product at 1024 x 1024.)
-    if (!producer) {
+// 256 x 128 tiles by eight waves of 64 x 64, two per SIMD, one workgroup per CU; three K-tile
+// buffers, the requests two K-tiles ahead, one barrier per K-tile.
+//
+// What bounds it: 8192 x 4096 runs at 1.2 PFLOP/s of matrix work, a library product of 8192^3 in
+// fp16 at 1.29. With its matrix instructions alone (registers that do not change) the loop
+// reaches 1.54, its LDS-DMA alone would allow 2.0 and its LDS reads alone 4. Three other schedules
+// of the same products ended within 3 % of this one: 128 x 128 tiles on two workgroups per CU,
+// waves half a K-tile apart (one half reads while the other multiplies), and fragments read ahead
+// behind a barrier in the middle of a K-tile. Four waves of 64 x 64 or 128 x 64, one per SIMD, with
+// two sets of fragments were 4 to 10 % slower.
+template <typename E, int TO, bool MUON>
+__device__ __forceinline__ void ns_wide_body(const NsArgs& args, int step, float ca, float cb,
+                                             float cc, const NsMuon& mo) {
+  constexpr int BM = 256, BN = 128, NI = 4, NB = 3;
+  constexpr int P_BYTES = BM * 128, BUF_BYTES = P_BYTES + BN * 128;
+  constexpr int RP = 4, RQ = 2, R = RP + RQ;    // requests per wave and K-tile
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave >> 1, wc = wave & 1;
+  NsTile w;
+  if (!ns_locate<BM, BN, TO>(args, step, w)) return;
+  const NsMat& t = args.t[w.mat];
+  const long pitch = pitch_of(w.K);
+
+  // piece r of an operand: rows 8 (8 r + wave) .. + 7
+  unsigned voff_p[RP], voff_q[RQ];
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+  for (int r = 0; r < RP; ++r) {
+    const int row = (r * 8 + wave) * 8 + (lane >> 3), kc = (lane & 7) ^ ((row >> 1) & 7);
+    voff_p[r] = (unsigned)(w.m0 + row < w.M ? row : w.M - 1 - w.m0) * (unsigned)pitch + 16u * kc;
+  }
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
+  for (int r = 0; r < RQ; ++r) {
+    const int row = (r * 8 + wave) * 8 + (lane >> 3), kc = (lane & 7) ^ ((row >> 1) & 7);
+    voff_q[r] = (unsigned)(w.n0 + row < w.N ? row : w.N - 1 - w.n0) * (unsigned)pitch + 16u * kc;
+  }
+  const __amdgpu_buffer_rsrc_t p_rsrc = rows_rsrc(w.P + w.m0 * pitch);
+  const __amdgpu_buffer_rsrc_t q_rsrc = rows_rsrc(w.Q + w.n0 * pitch);
+  // (behind the last K-tile the last one again, into a buffer nobody reads: the counts of the
+  // waits stay the same)
+  auto request = [&](int r, int kt, char* buf) {
+    const int at = (w.kt0 + (kt < w.nkt ? kt : w.nkt - 1)) * 128;
+    if (r < RP)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(p_rsrc, (lds_void*)(buf + (r * 8 + wave) * 1024), 16,
+                                               voff_p[r], at, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          q_rsrc, (lds_void*)(buf + P_BYTES + ((r - RP) * 8 + wave) * 1024), 16, voff_q[r - RP], at,
+          0, 0);
+  };
+  const int frow = lane & 15, fq = lane >> 4;
+  const int p_hi = piece_off(wr * 64 + frow, fq), p_lo = piece_off(wr * 64 + frow, 4 + fq);
+  const int q_hi = P_BYTES + piece_off(wc * 64 + frow, fq);
+  const int q_lo = P_BYTES + piece_off(wc * 64 + frow, 4 + fq);
+  auto fragment = [&](const char* at, int i) {   // (16 rows further: the same swizzle)
+    return *reinterpret_cast<const f16x8*>(at + i * 2048);
+  };
+  f32x4 sum[NI][NI], acc[NI][NI];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const pair_t v = (pair_t)__float_as_uint(sum[i][j][2 * h]) |
-                             (pair_t)__float_as_uint(sum[i][j][2 * h + 1]) << 32;
-            __hip_atomic_store(mine + ((i * NI + j) * 2 + h) * 256, v, __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
-          }
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int r = 0; r < R; ++r) request(r, k, smem + k * BUF_BYTES);
+  int cur = 0, free = 2 * BUF_BYTES;             // buffers of kt and kt + 2
+  // one K-tile; FIRST: the accumulators start from zero
+  auto multiply = [&](int kt, auto first) {
+    constexpr bool FIRST = decltype(first)::value;
+    // every wave's pieces of K-tile kt have landed (those of kt + 1 stay in flight), and every
+    // wave is done with the buffer before it
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(R) : "memory");
+    const char* buf = smem + cur;
+    f16x8 ph[NI], pl[NI], qh[NI], ql[NI];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) ql[j] = fragment(buf + q_lo, j);
+    ph[0] = fragment(buf + p_hi, 0);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) qh[j] = fragment(buf + q_hi, j);
+    pl[0] = fragment(buf + p_lo, 0);
+    // the order of the instructions is dealt out by hand: behind every four matrix instructions
+    // (one of the three products of a row of fragments) the next row's reads or a request
+#pragma unroll
+    for (int s = 0; s < 3 * NI; ++s) {
+      const int i = s / 3, term = s % 3;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        // (operands swapped: a lane's four results lie along N)
+        const f32x4 from = FIRST && term == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j];
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            term == 0 ? ql[j] : qh[j], term == 1 ? pl[i] : ph[i], from, 0, 0, 0);
+      }
+      if (term == 0 && i + 1 < NI) {
+        ph[i + 1] = fragment(buf + p_hi, i + 1);
+        pl[i + 1] = fragment(buf + p_lo, i + 1);
+      }
+      if (s % 2 == 1) request(s / 2, kt + 2, smem + free);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's part has arrived ...
-    __syncthreads();                                   // ... and every wave's, before the count
-    if (tid == 0) {
-      const int before = __hip_atomic_fetch_add(&args.arrived[shared_tile], 1, __ATOMIC_RELAXED,
-                                                __HIP_MEMORY_SCOPE_AGENT);
-      last = before == splits - 1;
-      if (last)                                 // nobody else comes: ready for the next launch
-        __hip_atomic_store(&args.arrived[shared_tile], 0, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!last || producer) return;
-    pair_t* all = reinterpret_cast<pair_t*>(args.partial) +
-                  (long)shared_tile * args.splits * PAIRS + tid;
+    free = cur;
+    cur = cur + BUF_BYTES == NB * BUF_BYTES ? 0 : cur + BUF_BYTES;
+  };
+  for (int base = 0; base < w.nkt; base += NS_CHAIN) {
+    multiply(base, yes());
+    const int end = base + NS_CHAIN < w.nkt ? base + NS_CHAIN : w.nkt;
+    for (int kt = base + 1; kt < end; ++kt) multiply(kt, no());
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < splits; ++k) {
-      pair_t v[NI][NI][2];
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            v[i][j][h] = __hip_atomic_load(all + ((i * NI + j) * 2 + h) * 256, __ATOMIC_RELAXED,
-                                           __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            sum[i][j][r] += __uint_as_float((unsigned)(v[i][j][r >> 1] >> (32 * (r & 1))));
-      all += PAIRS;
-    }
+      for (int j = 0; j < NI; ++j) sum[i][j] += acc[i][j];
   }
-  auto& acc = sum;
-
-  // lane: rows mb + 16 i, columns nb + 16 j + 0..3
-  const int mb = m0 + wr * WT + frow, nb = n0 + wc * WT + 4 * fq;
-  if (TO == TO_OUT) {
-    const float lr = MUON ? (mo.lr_dev ? mo.lr_dev[0] : mo.lr) : 0.f;
-    const float keep = 1.f - lr * mo.decay, take = lr * t.scale;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int m = mb + 16 * i;
-      if (m >= M) continue;
-      E* row = (E*)t.out + (long)m * N;
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const int n = nb + 16 * j;
-        if (n >= N) continue;
-        float v[4], w[4];
-        if (MUON) load_part<4>(row, n, N, w);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          v[r] = acc[i][j][r] * (1.f / (X_SCALE * AB_SCALE));
-          if (MUON) v[r] = __builtin_fmaf(-take, v[r], keep * w[r]);
-        }
-        store_part<4>(row, n, N, v);
-      }
-    }
-    return;
-  }
-
-  // packed (hi | lo << 16) results; zero behind the last row and column
-  unsigned pk[NI][NI][4];
-#pragma unroll
-  for (int i = 0; i < NI; ++i)
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int m = mb + 16 * i, n = nb + 16 * j;
-      f32x4 v = acc[i][j];
-      if (TO == TO_A) v *= AB_SCALE / (X_SCALE * X_SCALE);
-      if (TO == TO_X) v *= 1.f / AB_SCALE;
-      if (TO == TO_B) {
-        f16x4 ah = {0, 0, 0, 0}, al = {0, 0, 0, 0};
-        if (m < M && (n & ~31) < N) {
-          const char* src = t.a + m * pitch + split_off(n);
-          ah = *reinterpret_cast<const f16x4*>(src);
-          al = *reinterpret_cast<const f16x4*>(src + 64);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          v[r] = __builtin_fmaf(cc / AB_SCALE, v[r],
-                                __builtin_fmaf(cb, (float)ah[r] + (float)al[r],
-                                               m == n + r ? ca * AB_SCALE : 0.f));
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        pk[i][j][r] = m < M && n + r < N ? split_pack(v[r]) : 0u;
-    }
-
-  char* direct = TO == TO_A ? t.a : TO == TO_B ? t.b : t.x;          // rows along M
-  char* turned = TO == TO_X ? ((step & 1) ? t.xt0 : t.xt1) : direct;   // rows along N
-  const long d_pitch = 4L * (TO == TO_X ? t.kn : t.km), e_pitch = 4L * t.km;
-#pragma unroll
-  for (int i = 0; i < NI; ++i)
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int m = mb + 16 * i, n = nb + 16 * j;
-      if (m < M && (n & ~31) < N) {
-        char* dst = direct + m * d_pitch + split_off(n);
-        const unsigned* p = pk[i][j];
-        *reinterpret_cast<uint2*>(dst) = uint2{(p[0] & 0xffffu) | p[1] << 16,
-                                               (p[2] & 0xffffu) | p[3] << 16};
-        *reinterpret_cast<uint2*>(dst + 64) = uint2{p[0] >> 16 | (p[1] & 0xffff0000u),
-                                                    p[2] >> 16 | (p[3] & 0xffff0000u)};
-      }
-    }
-  if ((TO == TO_A || TO == TO_B) && tm == tn) return;   // a diagonal tile is its own mirror image
-  // the other order through a strip of LDS per wave: [WT of N][32 of M], rows of 36 dwords
-  unsigned* strip = reinterpret_cast<unsigned*>(smem) + wave * (WT * 36);
-#pragma unroll
-  for (int h = 0; h < NI / 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          strip[(16 * j + 4 * fq + r) * 36 + 16 * i + frow] = pk[2 * h + i][j][r];
-    __builtin_amdgcn_wave_barrier();
-    const int mc = m0 + wr * WT + 32 * h;               // first element of the chunk
-#pragma unroll
-    for (int q = 0; q < NI; ++q) {
-      const int nl = 16 * q + (lane >> 2), n = n0 + wc * WT + nl;
-      unsigned p[8];
-      const u32x4* src = reinterpret_cast<const u32x4*>(strip + nl * 36 + (lane & 3) * 8);
-      *reinterpret_cast<u32x4*>(p) = src[0];
-      *reinterpret_cast<u32x4*>(p + 4) = src[1];
-      if (n < N && mc < M) store_split8(turned + n * e_pitch + split_off(mc + (lane & 3) * 8), p);
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
+  // the buffers become the epilogue's scratch
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if (w.splits > 1 && !ns_join<NI, NI, 512>(sum, args, w)) return;
+  ns_store<E, NI, NI, TO, MUON>(sum, t, w, step, ca, cb, cc, mo, w.m0 + wr * 64, w.n0 + wc * 64,
+                                reinterpret_cast<unsigned*>(smem) + wave * (64 * 36));
 }
 
-// 64 x 64 tiles: with request-issuing waves; 128 x 128: without. Two workgroups per CU either way.
+// T = 64: 64 x 64 tiles; 256: 256 x 128
 template <typename E, int T, int TO, bool MUON>
-__global__ __launch_bounds__(T == 64 ? 512 : 256, T == 64 ? 4 : 2) void ns_product_kernel(
+__global__ __launch_bounds__(512, T == 64 ? 4 : 2) void ns_product_kernel(
     NsArgs args, int step, float ca, float cb, float cc, NsMuon mo) {
-  ns_product_body<E, T, TO, MUON, T == 64>(args, step, ca, cb, cc, mo);
+  if constexpr (T == 64)
+    ns_small_body<E, TO, MUON>(args, step, ca, cb, cc, mo);
+  else
+    ns_wide_body<E, TO, MUON>(args, step, ca, cb, cc, mo);
 }
 
 #include "newton_schulz_thin.h"
@@ -617,15 +759,17 @@ NsSizes sizes_of(long rows, long cols) {
   s.kn = up(s.n, 32);
   const long want = (rows * cols + 4095) / 4096;
   s.parts = want < NS_MAX_PARTS ? want : NS_MAX_PARTS;
-  s.x = up(4 * s.m * s.kn, 256);
-  s.xt = up(4 * s.n * s.km, 256);
-  s.sq = up(4 * s.m * s.km, 256);
+  s.x = up(s.m * pitch_of((int)s.kn), 256);
+  s.xt = up(s.n * pitch_of((int)s.km), 256);
+  s.sq = up(s.m * pitch_of((int)s.km), 256);
   s.total = up(8 * s.parts, 256) + s.x + 2 * s.xt + 2 * s.sq;
   return s;
 }
 
+// (a tile's rows lie within a 32-bit offset, 256 rows of 4 bytes an element; the tile counts of
+// 16 matrices within an int)
 bool bad_shape(long rows, long cols) {
-  return rows < 1 || cols < 1 || rows > (1L << 22) || cols > (1L << 22);
+  return rows < 1 || cols < 1 || rows > 4000000 || cols > 4000000 || rows * cols > (1L << 36);
 }
 
 // Sizes of X, A and B over the steps, from the singular values' side: s in [0, r] -> p(s) =
@@ -657,14 +801,35 @@ bool coefficients_fit(int steps, const float* coef) {
   return true;
 }
 
+// A tile size: its tiles, the workgroups of a product that run at once, LDS bytes, and what a
+// product costs: us per K-tile and CU, us per launch beside them
+struct NsShape {
+  int bm, bn, slots, lds;
+  float kt_us, launch_us;
+};
+NsShape shape_of(int tile) {
+  if (tile == 64) return {64, 64, 512, 4 * 2 * 64 * 128, 0.21f, 5.f};
+  return {256, 128, 256, 3 * 384 * 128, 1.0f, 10.f};
+}
+int full_tiles(const NsShape& s, int m, int n) {
+  return (m + s.bm - 1) / s.bm * ((n + s.bn - 1) / s.bn);
+}
+// (row tm of the triangle has bm / bn (tm + 1) tiles; the last row may have fewer columns)
+int triangle_tiles(const NsShape& s, int m) {
+  const int rows = (m + s.bm - 1) / s.bm, f = s.bm / s.bn;
+  return f * rows * (rows + 1) / 2 - (f * rows - (m + s.bn - 1) / s.bn);
+}
+
 // Which tiles of a product are split along K: those behind the last full round of the chip, as
 // many ways as the round has workgroups for.
-void plan_splits(NsArgs& args, int kt_max) {
-  const int tiles = args.first[args.count];
-  args.unsplit = tiles / NS_SLOTS * NS_SLOTS;
-  const int rest = tiles - args.unsplit;
-  args.splits = rest ? split_count(kt_max, NS_SLOTS / rest < 16 ? NS_SLOTS / rest : 16) : 1;
-  if (args.splits == 1) args.unsplit = tiles;
+void split_rule(const NsShape& shape, int tiles, int kt, int& unsplit, int& splits) {
+  unsplit = tiles / shape.slots * shape.slots;
+  const int rest = tiles - unsplit, most = rest ? shape.slots / rest : 1;
+  splits = split_count(kt, most < 16 ? most : 16);
+  if (splits == 1) unsplit = tiles;
+}
+void plan_splits(NsArgs& args, const NsShape& shape, int kt_max) {
+  split_rule(shape, args.first[args.count], kt_max, args.unsplit, args.splits);
 }
 unsigned grid_of(const NsArgs& args) {
   return args.unsplit + (args.first[args.count] - args.unsplit) * args.splits;
@@ -673,57 +838,94 @@ unsigned grid_of(const NsArgs& args) {
 template <typename E, int T, bool MUON>
 int launch_steps(const NsArgs& args, int steps, const float* coef, const NsMuon& mo,
                  hipStream_t stream) {
-  constexpr int LDS = (T == 64 ? 4 : 2) * 2 * T * 128;
-  static_assert(4 * (T / 2) * 36 * 4 <= LDS, "the epilogue's strips fit the K-tile buffers");
+  const NsShape shape = shape_of(T);
   static DtfPerDeviceOnce once;
   dtf_once_per_device(once, [&] {
-    allow_lds(ns_product_kernel<float, T, TO_A, false>, LDS);
-    allow_lds(ns_product_kernel<float, T, TO_B, false>, LDS);
-    allow_lds(ns_product_kernel<float, T, TO_X, false>, LDS);
-    allow_lds(ns_product_kernel<E, T, TO_OUT, MUON>, LDS);
+    allow_lds(ns_product_kernel<float, T, TO_A, false>, shape.lds);
+    allow_lds(ns_product_kernel<float, T, TO_B, false>, shape.lds);
+    allow_lds(ns_product_kernel<float, T, TO_X, false>, shape.lds);
+    allow_lds(ns_product_kernel<E, T, TO_OUT, MUON>, shape.lds);
   });
-  NsArgs sym = args, full = args;
+  // (the last product's tiles lie along the caller's rows)
+  NsArgs sym = args, full = args, last = args;
   int km = 0, kn = 0;
   for (int i = 0; i < args.count; ++i) {
-    const int tm = (args.t[i].m + T - 1) / T, tn = (args.t[i].n + T - 1) / T;
-    sym.first[i + 1] = sym.first[i] + tm * (tm + 1) / 2;
-    full.first[i + 1] = full.first[i] + tm * tn;
-    km = args.t[i].km > km ? args.t[i].km : km;
-    kn = args.t[i].kn > kn ? args.t[i].kn : kn;
+    const NsMat& t = args.t[i];
+    const bool tall = t.rows > t.cols;
+    sym.first[i + 1] = sym.first[i] + triangle_tiles(shape, t.m);
+    full.first[i + 1] = full.first[i] + full_tiles(shape, t.m, t.n);
+    last.first[i + 1] = last.first[i] + full_tiles(shape, tall ? t.n : t.m, tall ? t.m : t.n);
+    km = t.km > km ? t.km : km;
+    kn = t.kn > kn ? t.kn : kn;
   }
   NsArgs square = sym;
-  plan_splits(sym, kn / 32);
-  plan_splits(square, km / 32);
-  plan_splits(full, km / 32);
-  const dim3 block(T == 64 ? 512 : 256);
+  plan_splits(sym, shape, kn / 32);
+  plan_splits(square, shape, km / 32);
+  plan_splits(full, shape, km / 32);
+  plan_splits(last, shape, km / 32);
+  const dim3 block(512);
   for (int k = 0; k < steps; ++k) {
     const float a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
-    hipLaunchKernelGGL((ns_product_kernel<float, T, TO_A, false>), dim3(grid_of(sym)), block, LDS, stream,
-                       sym, k, a, b, c, mo);
-    hipLaunchKernelGGL((ns_product_kernel<float, T, TO_B, false>), dim3(grid_of(square)), block, LDS,
-                       stream, square, k, a, b, c, mo);
+    hipLaunchKernelGGL((ns_product_kernel<float, T, TO_A, false>), dim3(grid_of(sym)), block,
+                       shape.lds, stream, sym, k, a, b, c, mo);
+    hipLaunchKernelGGL((ns_product_kernel<float, T, TO_B, false>), dim3(grid_of(square)), block,
+                       shape.lds, stream, square, k, a, b, c, mo);
     if (k + 1 < steps)
-      hipLaunchKernelGGL((ns_product_kernel<float, T, TO_X, false>), dim3(grid_of(full)), block, LDS,
-                         stream, full, k, a, b, c, mo);
+      hipLaunchKernelGGL((ns_product_kernel<float, T, TO_X, false>), dim3(grid_of(full)), block,
+                         shape.lds, stream, full, k, a, b, c, mo);
     else
-      hipLaunchKernelGGL((ns_product_kernel<E, T, TO_OUT, MUON>), dim3(grid_of(full)), block, LDS,
-                         stream, full, k, a, b, c, mo);
+      hipLaunchKernelGGL((ns_product_kernel<E, T, TO_OUT, MUON>), dim3(grid_of(last)), block,
+                         shape.lds, stream, last, k, a, b, c, mo);
   }
   DTF_LAUNCH_CHECK();
   return DTF_OK;
 }
 
-// tile size of a call: 128 once that many tiles give the chip's 256 CUs two workgroups each
-int tile_of(long tiles128) { return tiles128 >= NS_SLOTS ? 128 : 64; }
+// us of one product under the split rule: K-tiles that the busiest CU goes through
+float product_us(const NsShape& shape, int tiles, int kt) {
+  int unsplit, splits;
+  split_rule(shape, tiles, kt, unsplit, splits);
+  const int items = (tiles - unsplit) * splits, cus = 256;
+  float us = shape.launch_us + (unsplit + cus - 1) / cus * kt * shape.kt_us;
+  if (splits > 1) us += (items + cus - 1) / cus * (kt / splits) * shape.kt_us + 8.f;
+  return us;
+}
 
-// (thin matrices have no tiles)
-long tiles128_of(long rows, long cols) {
-  return is_thin(rows, cols) ? 0 : ((rows + 127) / 128) * ((cols + 127) / 128);
+// Tile size of a call: the one whose three products take less time by the figures above. Measured
+// (64 x 64 / 256 x 128, us a call): 1024 x 1024 195 / 644, eight of them 798 / 780, 2048 x 2048 743 /
+// 935, 2560 x 2560 1547 / 1201, 2048 x 4096 1200 / 1135, 1024 x 8192 617 / 865, 4096 x 4096 5669 /
+// 3775.
+int tile_of(int count, const int* rows, const int* cols) {
+  int best = 64;
+  float least = 0.f;
+  for (int tile : {64, 256}) {
+    const NsShape s = shape_of(tile);
+    int full = 0, square = 0, km = 0, kn = 0;
+    for (int i = 0; i < count; ++i) {
+      if (is_thin(rows[i], cols[i])) continue;
+      const int m = rows[i] < cols[i] ? rows[i] : cols[i], n = rows[i] < cols[i] ? cols[i] : rows[i];
+      full += full_tiles(s, m, n);
+      square += triangle_tiles(s, m);
+      km = m > km ? m : km;
+      kn = n > kn ? n : kn;
+    }
+    const int bt = (km + 31) / 32, at = (kn + 31) / 32;
+    const float us =
+        product_us(s, full, bt) + product_us(s, square, bt) + product_us(s, square, at);
+    if (tile == 64 || us < least) {
+      best = tile;
+      least = us;
+    }
+  }
+  return best;
 }
 
 // head of the workspace: arrival counts, then the partial tiles of one split product
 constexpr long NS_HEAD = 4L * NS_SLOTS;
-long shared_bytes(int tile) { return NS_HEAD + 4L * NS_SLOTS * tile * tile; }
+long shared_bytes(int tile) {
+  const NsShape s = shape_of(tile);
+  return NS_HEAD + 4L * s.slots * s.bm * s.bn;
+}
 
 template <typename E, bool MUON>
 int launch(const NsArgs& args, const NsArgs& parts, const NsArgs& split, const NsArgs& thin,
@@ -740,8 +942,8 @@ int launch(const NsArgs& args, const NsArgs& parts, const NsArgs& split, const N
   hipLaunchKernelGGL((ns_split_kernel<E, MUON>), dim3(split.first[n]), dim3(256), 0, stream, split,
                      eps, mo);
   DTF_LAUNCH_CHECK();
-  return tile == 128 ? launch_steps<E, 128, MUON>(args, steps, coef, mo, stream)
-                     : launch_steps<E, 64, MUON>(args, steps, coef, mo, stream);
+  if (tile == 64) return launch_steps<E, 64, MUON>(args, steps, coef, mo, stream);
+  return launch_steps<E, 256, MUON>(args, steps, coef, mo, stream);
 }
 
 template <bool MUON>
@@ -758,13 +960,14 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
   NsArgs args = {}, thin = {};
   char* at = (char*)workspace;
   if ((uintptr_t)at & 255) return DTF_ERR_BAD_ARG;
-  long used = 0, tiles128 = 0;
+  long used = 0;
+  bool tiled = false;
   for (int i = 0; i < count; ++i) {
     if (bad_shape(rows[i], cols[i])) return DTF_ERR_BAD_ARG;
-    tiles128 += tiles128_of(rows[i], cols[i]);
+    tiled = tiled || !is_thin(rows[i], cols[i]);
   }
-  const int tile = tile_of(tiles128);
-  if (tiles128 > 0) {
+  const int tile = tile_of(count, rows, cols);
+  if (tiled) {
     args.arrived = (int*)at;
     args.partial = (float*)(at + NS_HEAD);
     at += shared_bytes(tile);
@@ -836,13 +1039,14 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
 // bytes of workspace (256-byte aligned) for `count` matrices; 0 for shapes that are not taken
 DTF_API long dtf_newton_schulz_workspace(int count, const int* rows, const int* cols) {
   if (count < 0 || count > NS_MAX_MATS || (count > 0 && (!rows || !cols))) return 0;
-  long total = 256, tiles128 = 0;
+  long total = 256;
+  bool tiled = false;
   for (int i = 0; i < count; ++i) {
     if (bad_shape(rows[i], cols[i])) return 0;
-    tiles128 += tiles128_of(rows[i], cols[i]);
+    tiled = tiled || !is_thin(rows[i], cols[i]);
     total += sizes_of(rows[i], cols[i]).total;
   }
-  return total + (tiles128 ? shared_bytes(tile_of(tiles128)) : 0);
+  return total + (tiled ? shared_bytes(tile_of(count, rows, cols)) : 0);
 }
 
 // out[i] = orthogonalised g[i], both [rows[i], cols[i]] contiguous of `type` (0 fp32, 1 bf16,

@@ -1316,7 +1316,7 @@ def _ns_workspace(shapes, device, what: str):
     cols = (ctypes.c_int * n)(*[s[1] for s in shapes])
     size = lib().dtf_newton_schulz_workspace(n, rows, cols)
     if size <= 0:
-        raise HipKernelError("%s: matrices of up to 2^22 rows and columns, got %s"
+        raise HipKernelError("%s: matrices of up to 4000000 rows and columns, got %s"
                              % (what, list(shapes)))
     ws = torch.empty((size,), dtype=torch.uint8, device=device)
     base = (ws.data_ptr() + 255) // 256 * 256
@@ -1416,13 +1416,17 @@ def multi_muon(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         if p.numel() == 0:
             continue
         g = g if g.is_contiguous() else g.contiguous()
-        spans += [(t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in (p, m)]
+        spans += [(t.data_ptr(), t.data_ptr() + 4 * t.numel(), writes)
+                  for t, writes in ((p, True), (m, True), (g, False))]
         scale = float(scales[i]) if scales is not None else muon_scale(*p.shape[-2:])
         work += [(a, b, c, scale) for a, b, c in
                  (zip(p, g, m) if p.dim() == 3 else ((p, g, m),))]
-    spans.sort()
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-        raise HipKernelError("multi_muon: params and moments overlap in memory")
+    written = read = 0                # how far the memory of the ones before reaches
+    for lo, hi, writes in sorted(spans):
+        if lo < written or writes and lo < read:
+            raise HipKernelError("multi_muon: params and moments overlap in memory, or a gradient "
+                                 "lies in one of them")
+        written, read = (max(written, hi), read) if writes else (written, max(read, hi))
     if lr_dev is not None and work and lr_dev.device != work[0][0].device:
         raise HipKernelError("multi_muon: lr is on another device")
     c = ctypes

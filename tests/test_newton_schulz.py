@@ -136,7 +136,7 @@ def hip():
     return h
 
 
-# both sides of the 32-element chunks, the 64- and 128-wide tiles; vectors; wide and tall
+# both sides of the 32-element chunks and the 64-wide tiles; thin ones; vectors; wide and tall
 SHAPES = [(1, 1), (1, 2), (2, 1), (3, 3), (1, 300), (300, 1), (7, 31), (32, 32), (33, 32), (31, 65),
           (63, 64), (64, 65), (65, 129), (100, 10), (784, 100), (100, 784), (127, 128), (129, 500),
           (300, 301), (515, 1030)]
@@ -157,6 +157,56 @@ def test_newton_schulz_matches_64_bits(hip, rows, cols, kind, dtype):
 def test_large_matrices(hip, rows, cols, dtype):
     g = _matrix(rows, cols, "low_rank").to(dtype).cuda()
     _check(hip.newton_schulz(g, steps=3), g, dtype, steps=3)
+
+
+# (as many as it takes for the 256 x 128 tiles; odd edges on each side of them, wide and tall)
+MANY = [(1001, 1003), (1003, 1001), (1009, 1011), (1024, 1021), (997, 1020), (1020, 999),
+        (1018, 1023), (1010, 1009)]
+MANY += [(c, r) for r, c in MANY[:7]] + [(70, 900)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_many_large_matrices(hip, dtype):
+    mats = [_matrix(r, c, ("low_rank", "gauss")[i % 2]).to(dtype).cuda()
+            for i, (r, c) in enumerate(MANY)]
+    outs = hip.newton_schulz(mats, steps=3)
+    for g, out, again in zip(mats, outs, hip.newton_schulz(mats, steps=3)):
+        assert torch.equal(out, again)
+        _check(out, g, dtype, steps=3)
+
+
+@pytest.mark.gpu
+def test_muon_of_many_large_matrices(hip):
+    gs = [_matrix(r, c).cuda() for r, c in MANY]
+    ws = [_matrix(r, c, seed=1).cuda() for r, c in MANY]
+    vs = [_matrix(r, c, seed=2).cuda() for r, c in MANY]
+    want = [muon_exact(w, g, v, 0.05, steps=3, decay=0.1) for w, g, v in zip(ws, gs, vs)]
+    tops = [w.abs().max().item() for w in ws]
+    hip.multi_muon(ws, gs, vs, 0.05, steps=3, weight_decay=0.1)
+    for w, (ew, _, u), top in zip(ws, want, tops):
+        s = max(1.0, w.shape[1] / w.shape[0]) ** 0.5
+        tol = 0.05 * s * _spectral_bound(u, 3) + 4 * 2.0 ** -24 * (top + 0.05 * s)
+        assert (w.double().cpu() - ew).abs().max().item() <= tol
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(hip):
+    """Calls that run side by side have workspaces and arrival counts of their own."""
+    sets = [[_matrix(300, 8000, seed=i).cuda()] if i % 2 else
+            [_matrix(1024, 1024, seed=i).cuda(), _matrix(50, 70, seed=i).cuda()] for i in range(4)]
+    want = [hip.newton_schulz(s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[] for _ in sets]
+    for _ in range(5):
+        for s, stream, out in zip(sets, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(hip.newton_schulz(s))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(w, out))
 
 
 @pytest.mark.gpu
@@ -273,10 +323,17 @@ def test_multi_muon_stacks_scales_and_refusals(hip):
     a, b, c = m.clone(), m.clone(), m.clone()
     hip.multi_muon([torch.empty(0, 4, device="cuda")], [torch.empty(0, 4, device="cuda")],
                    [torch.empty(0, 4, device="cuda")], 0.1)
+    # (one gradient of two weights is fine)
+    p, q, r = torch.zeros_like(m), torch.zeros_like(m), torch.randn(4, 5, generator=gen).cuda()
+    hip.multi_muon([p, q], [r, r], [torch.zeros_like(m), torch.zeros_like(m)], 0.1)
+    assert torch.equal(p, q) and p.abs().max() > 0
     for call in (lambda: hip.multi_muon([a], [b], [], 0.1),
                  lambda: hip.multi_muon([a], [b], [c], 0.1, scales=[]),
                  lambda: hip.multi_muon([a], [b], [a], 0.1),
                  lambda: hip.multi_muon([a, a], [b, b], [c, m], 0.1),
+                 lambda: hip.multi_muon([a], [a], [c], 0.1),
+                 lambda: hip.multi_muon([a], [c], [c], 0.1),
+                 lambda: hip.multi_muon([a, b], [m, a], [c, torch.zeros_like(m)], 0.1),
                  lambda: hip.multi_muon([a.t()], [b.t()], [c.t()], 0.1),
                  lambda: hip.multi_muon([a], [b.t()], [c], 0.1),
                  lambda: hip.multi_muon([a[0]], [b[0]], [c[0]], 0.1),
