@@ -20,8 +20,10 @@
 // Work. A and B are symmetric: only tiles on and below the diagonal are computed, each written
 // to both places. a I is part of B, so X is not read again for the sum. B X needs the columns of
 // X where A = X X^T needs its rows: the epilogue that makes X writes it in both orders, and all
-// operands are K-contiguous. The matrices of one call (up to NS_MAX_MATS, any shapes) share each
-// launch: a call takes 2 + 3 steps launches whatever the count.
+// operands are K-contiguous. Long matrices take two steps as one (step_pairs), which leaves out
+// every other pair of products with X. The matrices of one call (up to NS_MAX_MATS, any shapes)
+// share each launch: two, and three per step, whatever the count; long ones may have a sequence of
+// their own, and matrices of up to 64 rows or columns have (newton_schulz_thin.h).
 //
 // Layout. "Split rows": row r of K elements takes 4 bytes per element, in chunks of 32 elements:
 // 32 hi halves (64 bytes), then 32 lo halves. A chunk is 128 bytes, so a K-tile of 32 elements has
@@ -52,7 +54,7 @@ struct no {
 };
 
 enum { NS_F32 = 0, NS_BF16 = 1, NS_F16 = 2 };
-enum { TO_A = 0, TO_B = 1, TO_X = 2, TO_OUT = 3 };
+enum { TO_A = 0, TO_B = 1, TO_S = 2, TO_X = 3, TO_OUT = 4 };
 
 struct NsMat {
   const void* g;       // [rows, cols], contiguous
@@ -62,8 +64,7 @@ struct NsMat {
   char* x;             // split rows [m][kn]
   char* xt0;           // split rows [n][km]: read by even steps
   char* xt1;           //                     ... by odd ones
-  char* a;             // split rows [m][km]
-  char* b;
+  char* sq[3];         // split rows [m][km]: A, B and products of them
   int rows, cols;
   int m, n;
   int km, kn;          // m, n rounded up to whole chunks
@@ -79,6 +80,7 @@ struct NsArgs {
   // products: tiles [0, unsplit) have a workgroup each; every later tile has `splits`
   // workgroups that share its K range
   int unsplit, splits;
+  int p, q, to;                  // which of sq: first and second operand, result
   float* partial;                // [(tile - unsplit) * splits + split][T * T]
   int* arrived;                  // [tile - unsplit], zero between launches
 };
@@ -249,9 +251,10 @@ __device__ __forceinline__ int piece_off(int row, int kc) {
   return row * 128 + ((kc ^ ((row >> 1) & 7)) << 4);
 }
 
-// One BM x BN tile of P Q^T, P [M][K] and Q [N][K] in split rows. TO_A / TO_B: symmetric results
-// (M = N, tiles on and below the diagonal), written to both places; TO_X: written in both orders;
-// TO_OUT: the caller's type.
+// One BM x BN tile of P Q^T, P [M][K] and Q [N][K] in split rows. TO_A (X X^T), TO_B (a I + b A +
+// c A A) and TO_S (a product of polynomials of one A): symmetric results (M = N, tiles on and
+// below the diagonal), written to both places; TO_X: written in both orders; TO_OUT: the caller's
+// type.
 //
 // Accumulation. The matrix instruction adds its 32 products to the accumulator in steps of its
 // own; a long chain of them loses more than fp32 sums of rounded products do (1024 x 1024: the
@@ -292,15 +295,15 @@ __device__ __forceinline__ bool ns_locate(const NsArgs& args, int step, NsTile& 
   const int tile = id - args.first[w.mat];
   if (TO == TO_A) {
     w.P = w.Q = t.x; w.M = w.N = t.m; w.K = t.kn;
-  } else if (TO == TO_B) {
-    w.P = w.Q = t.a; w.M = w.N = t.m; w.K = t.km;
+  } else if (TO == TO_B || TO == TO_S) {
+    w.P = t.sq[args.p]; w.Q = t.sq[args.q]; w.M = w.N = t.m; w.K = t.km;
   } else {
     const char* xt = (step & 1) ? t.xt1 : t.xt0;
     w.K = t.km;
     if (TO == TO_OUT && t.rows > t.cols) {      // X^T = X^T B: the result as the caller lays it
-      w.P = xt; w.Q = t.b; w.M = t.n; w.N = t.m;
+      w.P = xt; w.Q = t.sq[args.p]; w.M = t.n; w.N = t.m;
     } else {
-      w.P = t.b; w.Q = xt; w.M = t.m; w.N = t.n;
+      w.P = t.sq[args.p]; w.Q = xt; w.M = t.m; w.N = t.n;
     }
   }
   const int all_kt = w.K / 32;
@@ -311,7 +314,7 @@ __device__ __forceinline__ bool ns_locate(const NsArgs& args, int step, NsTile& 
   w.kt0 = (int)((long)all_kt * w.split / w.splits);
   w.nkt = (int)((long)all_kt * (w.split + 1) / w.splits) - w.kt0;
   int tm, tn;
-  if (TO == TO_A || TO == TO_B) {
+  if (TO == TO_A || TO == TO_B || TO == TO_S) {
     // row tm of the triangle has F (tm + 1) tiles: F tm (tm + 1) / 2 before it
     constexpr int F = BM / BN;
     tm = (int)((__builtin_sqrtf(8.f / F * tile + 1.f) - 1.f) * 0.5f);
@@ -333,30 +336,26 @@ __device__ __forceinline__ bool ns_locate(const NsArgs& args, int step, NsTile& 
 
 // The parts of a shared tile. True in the workgroup that has all of them in `sum`. The XCDs' L2s
 // do not see each other's lines, so the parts go through memory: stores and loads of device scope
-// pass the L2 by, and a store is complete once it has arrived there. (A release fence instead
+// (sc1) pass the L2 by, and a store is complete once it has arrived there. (A release fence instead
 // writes the whole L2 back, 0.4 us each and one after the other on an XCD: 29 us for a product at
-// 1024 x 1024 split three ways.) The first THREADS threads hold the tile.
+// 1024 x 1024 split three ways.) The first THREADS threads hold the tile. A load from there takes
+// a microsecond and more, so 8 of a thread's are on their way at once, and as many again are asked
+// for before the first are added.
+constexpr int SC1 = 16;
 template <int NM, int NN, int THREADS>
 __device__ __forceinline__ bool ns_join(f32x4 (&sum)[NM][NN], const NsArgs& args, const NsTile& w) {
   __shared__ int last;
-  constexpr int PAIRS = NM * NN * 2 * THREADS;  // 8-byte pairs in a partial tile
+  constexpr int FR = NM * NN, PART = FR * THREADS * 16;      // fragments and bytes of a part
+  constexpr int U = 16 / FR;                                 // parts in two requests of 8 loads
   const bool holds = threadIdx.x < THREADS;
-  typedef unsigned long long pair_t;
-  pair_t* part = reinterpret_cast<pair_t*>(args.partial) + (long)w.shared * args.splits * PAIRS +
-                 threadIdx.x;
+  const __amdgpu_buffer_rsrc_t parts =
+      rows_rsrc((const char*)args.partial + (long)w.shared * args.splits * PART);
+  const int at = threadIdx.x * 16;
   if (holds) {
-    pair_t* mine = part + (long)w.split * PAIRS;
 #pragma unroll
-    for (int i = 0; i < NM; ++i)
-#pragma unroll
-      for (int j = 0; j < NN; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const pair_t v = (pair_t)__float_as_uint(sum[i][j][2 * h]) |
-                           (pair_t)__float_as_uint(sum[i][j][2 * h + 1]) << 32;
-          __hip_atomic_store(mine + ((i * NN + j) * 2 + h) * THREADS, v, __ATOMIC_RELAXED,
-                             __HIP_MEMORY_SCOPE_AGENT);
-        }
+    for (int f = 0; f < FR; ++f)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[f / NN][f % NN]),
+                                                 parts, at, w.split * PART + f * THREADS * 16, SC1);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's part has arrived ...
   __syncthreads();                                   // ... and every wave's, before the count
@@ -369,27 +368,31 @@ __device__ __forceinline__ bool ns_join(f32x4 (&sum)[NM][NN], const NsArgs& args
   }
   __syncthreads();
   if (!last || !holds) return false;
+  u32x4 v[2][8];
+  // half h of the loads of parts k .. k + U - 1 (behind the last part the last one again, not added)
+  auto ask = [&](int k, int h) {
 #pragma unroll
-  for (int i = 0; i < NM; ++i)
-#pragma unroll
-    for (int j = 0; j < NN; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < w.splits; ++k) {
-#pragma unroll
-    for (int i = 0; i < NM; ++i) {
-      pair_t v[NN][2];
-#pragma unroll
-      for (int j = 0; j < NN; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          v[j][h] = __hip_atomic_load(part + ((i * NN + j) * 2 + h) * THREADS, __ATOMIC_RELAXED,
-                                      __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-      for (int j = 0; j < NN; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          sum[i][j][r] += __uint_as_float((unsigned)(v[j][r >> 1] >> (32 * (r & 1))));
+    for (int x = 0; x < 8; ++x) {
+      const int part = k + (h * 8 + x) / FR, f = (h * 8 + x) % FR;
+      v[h][x] = __builtin_amdgcn_raw_buffer_load_b128(
+          parts, at, (part < w.splits ? part : w.splits - 1) * PART + f * THREADS * 16, SC1);
     }
-    part += PAIRS;
+  };
+  auto add = [&](int k, int h) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int f = (h * 8 + x) % FR;
+      if (k + (h * 8 + x) / FR < w.splits) sum[f / NN][f % NN] += __builtin_bit_cast(f32x4, v[h][x]);
+    }
+  };
+#pragma unroll
+  for (int f = 0; f < FR; ++f) sum[f / NN][f % NN] = f32x4{0.f, 0.f, 0.f, 0.f};
+  ask(0, 0);
+  for (int k = 0; k < w.splits; k += U) {
+    ask(k, 1);
+    add(k, 0);
+    if (k + U < w.splits) ask(k + U, 0);
+    add(k, 1);
   }
   return true;
 }
@@ -397,9 +400,10 @@ __device__ __forceinline__ bool ns_join(f32x4 (&sum)[NM][NN], const NsArgs& args
 // Results of one wave: rows mw + 16 i + lane % 16, columns nw + 16 j + 4 (lane / 16) + 0..3.
 // `strip`: 16 NN rows of 36 dwords of LDS, this wave's own.
 template <typename E, int NM, int NN, int TO, bool MUON>
-__device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsMat& t,
+__device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArgs& args,
                                          const NsTile& w, int step, float ca, float cb, float cc,
                                          const NsMuon& mo, int mw, int nw, unsigned* strip) {
+  const NsMat& t = args.t[w.mat];
   const int lane = threadIdx.x & 63, frow = lane & 15, fq = lane >> 4;
   const int mb = mw + frow, nb = nw + 4 * fq, M = w.M, N = w.N;
   if (TO == TO_OUT) {
@@ -426,11 +430,11 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsMat
     }
     return;
   }
-  constexpr bool SYM = TO == TO_A || TO == TO_B;
+  constexpr bool SYM = TO == TO_A || TO == TO_B || TO == TO_S;
   // (squares of this wave's size: above the diagonal the mirror image writes)
   const int row_block = mw / (16 * NM), col_block = nw / (16 * NN);
   if (SYM && row_block < col_block) return;
-  char* direct = TO == TO_A ? t.a : TO == TO_B ? t.b : t.x;            // rows along M
+  char* direct = SYM ? t.sq[args.to] : t.x;                            // rows along M
   char* turned = TO == TO_X ? ((step & 1) ? t.xt0 : t.xt1) : direct;   // rows along N
   const long d_pitch = pitch_of(TO == TO_X ? t.kn : t.km), t_pitch = pitch_of(t.km);
 #pragma unroll
@@ -444,14 +448,13 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsMat
         const int m = mb + 16 * (2 * h + i), n = nb + 16 * j;
         f32x4 v = acc[2 * h + i][j];
         if (TO == TO_A) v *= AB_SCALE / (X_SCALE * X_SCALE);
-        if (TO == TO_X) v *= 1.f / AB_SCALE;
+        if (TO == TO_X || TO == TO_S) v *= 1.f / AB_SCALE;
         if (TO == TO_B) {
-          f16x4 ah = {0, 0, 0, 0}, al = {0, 0, 0, 0};
-          if (m < M && (n & ~31) < N) {
-            const char* src = t.a + m * t_pitch + split_off(n);
-            ah = *reinterpret_cast<const f16x4*>(src);
-            al = *reinterpret_cast<const f16x4*>(src + 64);
-          }
+          // (any address inside for the elements that are not there: they become zeros below)
+          const char* src = t.sq[args.p] + (m < M ? m : 0) * t_pitch +
+                            split_off((n & ~31) < N ? n : 0);
+          const f16x4 ah = *reinterpret_cast<const f16x4*>(src);
+          const f16x4 al = *reinterpret_cast<const f16x4*>(src + 64);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             v[r] = __builtin_fmaf(cc / AB_SCALE, v[r],
@@ -508,7 +511,6 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
   const int wr = wave >> 1, wc = wave & 1;
   NsTile w;
   if (!ns_locate<T, T, TO>(args, step, w)) return;
-  const NsMat& t = args.t[w.mat];
   f32x4 sum[NI][NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -597,7 +599,7 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
   if (w.splits > 1 && !ns_join<NI, NI, 256>(sum, args, w)) return;
-  ns_store<E, NI, NI, TO, MUON>(sum, t, w, step, ca, cb, cc, mo, w.m0 + wr * WT, w.n0 + wc * WT,
+  ns_store<E, NI, NI, TO, MUON>(sum, args, w, step, ca, cb, cc, mo, w.m0 + wr * WT, w.n0 + wc * WT,
                                 reinterpret_cast<unsigned*>(smem) + wave * (WT * 36));
 }
 
@@ -623,7 +625,6 @@ __device__ __forceinline__ void ns_wide_body(const NsArgs& args, int step, float
   const int wr = wave >> 1, wc = wave & 1;
   NsTile w;
   if (!ns_locate<BM, BN, TO>(args, step, w)) return;
-  const NsMat& t = args.t[w.mat];
   const long pitch = pitch_of(w.K);
 
   // piece r of an operand: rows 8 (8 r + wave) .. + 7
@@ -717,7 +718,7 @@ __device__ __forceinline__ void ns_wide_body(const NsArgs& args, int step, float
   // the buffers become the epilogue's scratch
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   if (w.splits > 1 && !ns_join<NI, NI, 512>(sum, args, w)) return;
-  ns_store<E, NI, NI, TO, MUON>(sum, t, w, step, ca, cb, cc, mo, w.m0 + wr * 64, w.n0 + wc * 64,
+  ns_store<E, NI, NI, TO, MUON>(sum, args, w, step, ca, cb, cc, mo, w.m0 + wr * 64, w.n0 + wc * 64,
                                 reinterpret_cast<unsigned*>(smem) + wave * (64 * 36));
 }
 
@@ -762,7 +763,7 @@ NsSizes sizes_of(long rows, long cols) {
   s.x = up(s.m * pitch_of((int)s.kn), 256);
   s.xt = up(s.n * pitch_of((int)s.km), 256);
   s.sq = up(s.m * pitch_of((int)s.km), 256);
-  s.total = up(8 * s.parts, 256) + s.x + 2 * s.xt + 2 * s.sq;
+  s.total = up(8 * s.parts, 256) + s.x + 2 * s.xt + 3 * s.sq;
   return s;
 }
 
@@ -776,7 +777,8 @@ bool bad_shape(long rows, long cols) {
 // s q(s^2). The stored fp16 images must hold every entry, and an entry is at most the largest
 // singular value. The extremes of p and q lie at the ends and where a quadratic in t = s^2 has
 // its roots.
-bool coefficients_fit(int steps, const float* coef) {
+// `factor`: what step k multiplies a singular value by at most.
+bool coefficients_fit(int steps, const float* coef, double* factor) {
   double r = 1.0 + 1e-6;
   for (int k = 0; k < steps; ++k) {
     const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2], end = r * r;
@@ -796,20 +798,22 @@ bool coefficients_fit(int steps, const float* coef) {
     visit((-3.0 * b - root) / (10.0 * c));
     visit(-a / (3.0 * b));                       // ... with c = 0
     if (!(end <= AB_LIMIT) || !(q_top <= AB_LIMIT) || !(p_top <= X_LIMIT)) return false;
+    factor[k] = q_top;
     r = p_top * (1.0 + 1e-3);                    // (rounding of what is computed)
   }
   return true;
 }
 
-// A tile size: its tiles, the workgroups of a product that run at once, LDS bytes, and what a
-// product costs: us per K-tile and CU, us per launch beside them
+// A tile size: its tiles, the workgroups of a product that run at once, LDS bytes, and by
+// measurement what a product takes in us: per launch, for a K-tile in a workgroup that has the chip
+// to itself, for a K-tile of the whole chip's work, and for joining split tiles
 struct NsShape {
   int bm, bn, slots, lds;
-  float kt_us, launch_us;
+  float launch_us, alone_us, each_us, join_us;
 };
 NsShape shape_of(int tile) {
-  if (tile == 64) return {64, 64, 512, 4 * 2 * 64 * 128, 0.21f, 5.f};
-  return {256, 128, 256, 3 * 384 * 128, 1.0f, 10.f};
+  if (tile == 64) return {64, 64, 512, 4 * 2 * 64 * 128, 6.f, 0.23f, 0.0010f, 8.f};
+  return {256, 128, 256, 3 * 384 * 128, 14.f, 1.1f, 0.0051f, 24.f};
 }
 int full_tiles(const NsShape& s, int m, int n) {
   return (m + s.bm - 1) / s.bm * ((n + s.bn - 1) / s.bn);
@@ -828,122 +832,207 @@ void split_rule(const NsShape& shape, int tiles, int kt, int& unsplit, int& spli
   splits = split_count(kt, most < 16 ? most : 16);
   if (splits == 1) unsplit = tiles;
 }
-void plan_splits(NsArgs& args, const NsShape& shape, int kt_max) {
-  split_rule(shape, args.first[args.count], kt_max, args.unsplit, args.splits);
-}
-unsigned grid_of(const NsArgs& args) {
-  return args.unsplit + (args.first[args.count] - args.unsplit) * args.splits;
+// us of one product under the split rule: whole rounds of the chip, then what is behind them
+float product_us(const NsShape& shape, int tiles, int kt) {
+  int unsplit, splits;
+  split_rule(shape, tiles, kt, unsplit, splits);
+  auto round = [&](int items, int kts) {
+    const float one = kts * shape.alone_us, all = (float)items * kts * shape.each_us;
+    return items == 0 ? 0.f : one > all ? one : all;
+  };
+  const int whole = unsplit / shape.slots * shape.slots;
+  float us = shape.launch_us + round(whole, kt) + round(unsplit - whole, kt);
+  if (splits > 1) us += round((tiles - unsplit) * splits, kt / splits) + shape.join_us;
+  return us;
 }
 
+// The tile size that takes less time for a product; the wide one where they are close, because it
+// takes less power out of what the next product has. Measured (64 x 64 / 256 x 128, us): symmetric
+// products of 1024 x 1024 13 / 41, of 2048 x 2048 48 / 55, of 4096 x 4096 322 / 209; full ones of 1024 x
+// 1024 by 1024 x 4096 36 / 46, 2048 x 2048 by 2048 x 4096 142 / 95, 4096 x 4096 by 4096 x 8192 981 / 670.
+int faster_tile(const int (&tiles)[2], int kt, float& us) {
+  const float small = product_us(shape_of(64), tiles[0], kt);
+  const float wide = product_us(shape_of(256), tiles[1], kt);
+  us = small <= wide ? small : wide;
+  return 1.06f * small <= wide ? 64 : 256;
+}
+
+// How a call's tiled matrices are run: in one sequence of launches, or with those of n >= 5/4 m
+// in a sequence of their own that takes steps in pairs; and the tile size of each kind of product.
+struct NsTiles {
+  int gram, square, full;
+};
+struct NsPlan {
+  bool pairs;            // wide matrices apart
+  NsTiles tiles[2];      // of the sequence that takes single steps, of the other
+};
+bool is_wide(long rows, long cols) {
+  const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return 4 * n >= 5 * m;
+}
+// us of two steps on the matrices `which` picks (0: all, 1: wide ones, 2: the others)
+float steps_us(int count, const int* rows, const int* cols, int which, bool pairs, NsTiles& tiles) {
+  int full[2] = {0, 0}, square[2] = {0, 0}, km = 0, kn = 0;
+  for (int i = 0; i < count; ++i) {
+    if (is_thin(rows[i], cols[i]) || (which && is_wide(rows[i], cols[i]) != (which == 1))) continue;
+    const int m = rows[i] < cols[i] ? rows[i] : cols[i], n = rows[i] < cols[i] ? cols[i] : rows[i];
+    for (int k = 0; k < 2; ++k) {
+      full[k] += full_tiles(shape_of(k ? 256 : 64), m, n);
+      square[k] += triangle_tiles(shape_of(k ? 256 : 64), m);
+    }
+    km = m > km ? m : km;
+    kn = n > kn ? n : kn;
+  }
+  tiles = {64, 64, 64};
+  if (!km) return 0.f;
+  float g, q, f;
+  tiles.gram = faster_tile(square, (kn + 31) / 32, g);
+  tiles.square = faster_tile(square, (km + 31) / 32, q);
+  tiles.full = faster_tile(full, (km + 31) / 32, f);
+  return pairs ? g + 5.f * q + f : 2.f * (g + q + f);
+}
+NsPlan plan_of(int count, const int* rows, const int* cols) {
+  NsPlan one, apart;
+  const float whole = steps_us(count, rows, cols, 0, false, one.tiles[0]);
+  const float wide = steps_us(count, rows, cols, 1, true, apart.tiles[1]);
+  const float rest = steps_us(count, rows, cols, 2, false, apart.tiles[0]);
+  one.pairs = false;
+  one.tiles[1] = one.tiles[0];
+  apart.pairs = true;
+  return wide > 0.f && wide + rest < whole ? apart : one;
+}
+
+// Steps k and k + 1 taken as one. The second step's A is a polynomial of the first's, so X is
+// multiplied twice: A = X X^T, B = q(A), C = B A, A' = C B, B' = q'(A'), P = B' B, X = P X, where
+// single steps do it four times. For n = r m that is 3 r + 5 times m^3 instead of 6 r + 2 (2048 x
+// 8192 1.81 -> 1.40 ms, 8192 x 4096 6.46 -> 5.50, 1024 x 8192 0.60 -> 0.42). What is lost on A' acts on
+// P only through B', beside a I: five steps of 4096 x 8192 are off by 2.0e-6 (single steps 2.3e-6, an
+// fp32 computation 5.6e-6), of 1024 x 4096 with a quarter of the rank by 8.1e-6 (6.6e-6, 9.0e-6).
+// Three steps as one would lose a^2 as much again. Odd counts have their single step before the
+// last pair, where the singular values are least apart. P has to fit the images of B.
+bool step_pairs(int k, int steps, const double* factor) {
+  if (k + 1 >= steps || ((steps - k) % 2 && k + 3 >= steps)) return false;
+  return factor[k] * factor[k + 1] <= AB_LIMIT;
+}
+
+// matrices that go through the same launches
+struct NsSet {
+  NsArgs args;
+  NsTiles tiles;
+  bool pairs;
+};
+
+// One kind of product of a set: its tiles, and the launch of them
+struct NsLaunch {
+  NsArgs args;
+  NsShape shape;
+  template <typename Tiles>                      // tiles(shape, matrix)
+  NsLaunch(const NsSet& set, int tile, int kt_max, Tiles tiles)
+      : args(set.args), shape(shape_of(tile)) {
+    for (int i = 0; i < args.count; ++i) args.first[i + 1] = args.first[i] + tiles(shape, args.t[i]);
+    split_rule(shape, args.first[args.count], kt_max, args.unsplit, args.splits);
+  }
+  template <typename E, int TO, bool MUON>
+  void run(int p, int q, int to, int turn, const float* c, const NsMuon& mo, hipStream_t stream) {
+    args.p = p;
+    args.q = q;
+    args.to = to;
+    const unsigned grid =
+        args.unsplit + (args.first[args.count] - args.unsplit) * (unsigned)args.splits;
+    if (shape.bm == 64)
+      hipLaunchKernelGGL((ns_product_kernel<E, 64, TO, MUON>), dim3(grid), dim3(512), shape.lds,
+                         stream, args, turn, c[0], c[1], c[2], mo);
+    else
+      hipLaunchKernelGGL((ns_product_kernel<E, 256, TO, MUON>), dim3(grid), dim3(512), shape.lds,
+                         stream, args, turn, c[0], c[1], c[2], mo);
+  }
+};
+
 template <typename E, int T, bool MUON>
-int launch_steps(const NsArgs& args, int steps, const float* coef, const NsMuon& mo,
-                 hipStream_t stream) {
-  const NsShape shape = shape_of(T);
+void allow_product_lds() {
+  const int lds = shape_of(T).lds;
+  allow_lds(ns_product_kernel<float, T, TO_A, false>, lds);
+  allow_lds(ns_product_kernel<float, T, TO_B, false>, lds);
+  allow_lds(ns_product_kernel<float, T, TO_S, false>, lds);
+  allow_lds(ns_product_kernel<float, T, TO_X, false>, lds);
+  allow_lds(ns_product_kernel<E, T, TO_OUT, MUON>, lds);
+}
+
+template <typename E, bool MUON>
+int launch_steps(const NsSet& set, int steps, const float* coef, const double* factor,
+                 const NsMuon& mo, hipStream_t stream) {
   static DtfPerDeviceOnce once;
-  dtf_once_per_device(once, [&] {
-    allow_lds(ns_product_kernel<float, T, TO_A, false>, shape.lds);
-    allow_lds(ns_product_kernel<float, T, TO_B, false>, shape.lds);
-    allow_lds(ns_product_kernel<float, T, TO_X, false>, shape.lds);
-    allow_lds(ns_product_kernel<E, T, TO_OUT, MUON>, shape.lds);
+  dtf_once_per_device(once, [] {
+    allow_product_lds<E, 64, MUON>();
+    allow_product_lds<E, 256, MUON>();
   });
-  // (the last product's tiles lie along the caller's rows)
-  NsArgs sym = args, full = args, last = args;
   int km = 0, kn = 0;
-  for (int i = 0; i < args.count; ++i) {
-    const NsMat& t = args.t[i];
-    const bool tall = t.rows > t.cols;
-    sym.first[i + 1] = sym.first[i] + triangle_tiles(shape, t.m);
-    full.first[i + 1] = full.first[i] + full_tiles(shape, t.m, t.n);
-    last.first[i + 1] = last.first[i] + full_tiles(shape, tall ? t.n : t.m, tall ? t.m : t.n);
+  for (int i = 0; i < set.args.count; ++i) {
+    const NsMat& t = set.args.t[i];
     km = t.km > km ? t.km : km;
     kn = t.kn > kn ? t.kn : kn;
   }
-  NsArgs square = sym;
-  plan_splits(sym, shape, kn / 32);
-  plan_splits(square, shape, km / 32);
-  plan_splits(full, shape, km / 32);
-  plan_splits(last, shape, km / 32);
-  const dim3 block(512);
-  for (int k = 0; k < steps; ++k) {
-    const float a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
-    hipLaunchKernelGGL((ns_product_kernel<float, T, TO_A, false>), dim3(grid_of(sym)), block,
-                       shape.lds, stream, sym, k, a, b, c, mo);
-    hipLaunchKernelGGL((ns_product_kernel<float, T, TO_B, false>), dim3(grid_of(square)), block,
-                       shape.lds, stream, square, k, a, b, c, mo);
-    if (k + 1 < steps)
-      hipLaunchKernelGGL((ns_product_kernel<float, T, TO_X, false>), dim3(grid_of(full)), block,
-                         shape.lds, stream, full, k, a, b, c, mo);
+  const auto triangle = [](const NsShape& s, const NsMat& t) { return triangle_tiles(s, t.m); };
+  NsLaunch gram(set, set.tiles.gram, kn / 32, triangle);
+  NsLaunch square(set, set.tiles.square, km / 32, triangle);
+  NsLaunch full(set, set.tiles.full, km / 32,
+                [](const NsShape& s, const NsMat& t) { return full_tiles(s, t.m, t.n); });
+  // (the last product's tiles lie along the caller's rows)
+  NsLaunch last(set, set.tiles.full, km / 32,
+                [](const NsShape& s, const NsMat& t) { return full_tiles(s, t.rows, t.cols); });
+  for (int k = 0, turn = 0; k < steps; ++turn) {
+    const float* c = coef + 3 * k;
+    int at = 1;                                                                // factor of X
+    gram.run<float, TO_A, false>(0, 0, 0, turn, c, mo, stream);                // A
+    square.run<float, TO_B, false>(0, 0, 1, turn, c, mo, stream);              // B
+    if (set.pairs && step_pairs(k, steps, factor)) {
+      square.run<float, TO_S, false>(1, 0, 2, turn, c, mo, stream);            // C = B A
+      square.run<float, TO_S, false>(2, 1, 0, turn, c, mo, stream);            // A' = C B
+      square.run<float, TO_B, false>(0, 0, 2, turn, c + 3, mo, stream);        // B'
+      square.run<float, TO_S, false>(2, 1, 0, turn, c, mo, stream);            // P = B' B
+      at = 0;
+      ++k;
+    }
+    if (++k < steps)
+      full.run<float, TO_X, false>(at, 0, 0, turn, c, mo, stream);
     else
-      hipLaunchKernelGGL((ns_product_kernel<E, T, TO_OUT, MUON>), dim3(grid_of(last)), block,
-                         shape.lds, stream, last, k, a, b, c, mo);
+      last.run<E, TO_OUT, MUON>(at, 0, 0, turn, c, mo, stream);
   }
   DTF_LAUNCH_CHECK();
   return DTF_OK;
 }
 
-// us of one product under the split rule: K-tiles that the busiest CU goes through
-float product_us(const NsShape& shape, int tiles, int kt) {
-  int unsplit, splits;
-  split_rule(shape, tiles, kt, unsplit, splits);
-  const int items = (tiles - unsplit) * splits, cus = 256;
-  float us = shape.launch_us + (unsplit + cus - 1) / cus * kt * shape.kt_us;
-  if (splits > 1) us += (items + cus - 1) / cus * (kt / splits) * shape.kt_us + 8.f;
-  return us;
-}
-
-// Tile size of a call: the one whose three products take less time by the figures above. Measured
-// (64 x 64 / 256 x 128, us a call): 1024 x 1024 195 / 644, eight of them 798 / 780, 2048 x 2048 743 /
-// 935, 2560 x 2560 1547 / 1201, 2048 x 4096 1200 / 1135, 1024 x 8192 617 / 865, 4096 x 4096 5669 /
-// 3775.
-int tile_of(int count, const int* rows, const int* cols) {
-  int best = 64;
-  float least = 0.f;
-  for (int tile : {64, 256}) {
-    const NsShape s = shape_of(tile);
-    int full = 0, square = 0, km = 0, kn = 0;
-    for (int i = 0; i < count; ++i) {
-      if (is_thin(rows[i], cols[i])) continue;
-      const int m = rows[i] < cols[i] ? rows[i] : cols[i], n = rows[i] < cols[i] ? cols[i] : rows[i];
-      full += full_tiles(s, m, n);
-      square += triangle_tiles(s, m);
-      km = m > km ? m : km;
-      kn = n > kn ? n : kn;
-    }
-    const int bt = (km + 31) / 32, at = (kn + 31) / 32;
-    const float us =
-        product_us(s, full, bt) + product_us(s, square, bt) + product_us(s, square, at);
-    if (tile == 64 || us < least) {
-      best = tile;
-      least = us;
-    }
-  }
-  return best;
-}
-
 // head of the workspace: arrival counts, then the partial tiles of one split product
 constexpr long NS_HEAD = 4L * NS_SLOTS;
-long shared_bytes(int tile) {
-  const NsShape s = shape_of(tile);
+long shared_bytes(const NsPlan& plan) {
+  bool wide = false;
+  for (const NsTiles& t : plan.tiles)
+    wide = wide || t.gram != 64 || t.square != 64 || t.full != 64;
+  const NsShape s = shape_of(wide ? 256 : 64);
   return NS_HEAD + 4L * s.slots * s.bm * s.bn;
 }
 
 template <typename E, bool MUON>
-int launch(const NsArgs& args, const NsArgs& parts, const NsArgs& split, const NsArgs& thin,
-           int tile, int steps, const float* coef, float eps, const NsMuon& mo,
+int launch(const NsSet (&sets)[2], const NsArgs& parts, const NsArgs& split, const NsArgs& thin,
+           int steps, const float* coef, const double* factor, float eps, const NsMuon& mo,
            hipStream_t stream) {
   if (thin.count) {
     const int rc = launch_thin<E, MUON>(thin, steps, coef, eps, mo, stream);
     if (rc != DTF_OK) return rc;
   }
-  const int n = args.count;
+  const int n = parts.count;
   if (n == 0) return DTF_OK;
   hipLaunchKernelGGL((ns_norm_kernel<E, MUON>), dim3(parts.first[n]), dim3(256), 0, stream, parts,
                      mo);
   hipLaunchKernelGGL((ns_split_kernel<E, MUON>), dim3(split.first[n]), dim3(256), 0, stream, split,
                      eps, mo);
   DTF_LAUNCH_CHECK();
-  if (tile == 64) return launch_steps<E, 64, MUON>(args, steps, coef, mo, stream);
-  return launch_steps<E, 256, MUON>(args, steps, coef, mo, stream);
+  for (const NsSet& set : sets) {
+    if (set.args.count == 0) continue;
+    const int rc = launch_steps<E, MUON>(set, steps, coef, factor, mo, stream);
+    if (rc != DTF_OK) return rc;
+  }
+  return DTF_OK;
 }
 
 template <bool MUON>
@@ -955,7 +1044,8 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
       (count > 0 && (!g || !out || !rows || !cols || !workspace)))
     return DTF_ERR_BAD_ARG;
   if (count == 0) return DTF_OK;
-  if (!coefficients_fit(steps, coef)) return DTF_ERR_UNSUPPORTED;
+  double factor[NS_MAX_STEPS];
+  if (!coefficients_fit(steps, coef, factor)) return DTF_ERR_UNSUPPORTED;
   // thin matrices have kernels of their own; the others share the tiled sequence
   NsArgs args = {}, thin = {};
   char* at = (char*)workspace;
@@ -966,12 +1056,12 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     if (bad_shape(rows[i], cols[i])) return DTF_ERR_BAD_ARG;
     tiled = tiled || !is_thin(rows[i], cols[i]);
   }
-  const int tile = tile_of(count, rows, cols);
+  const NsPlan plan = plan_of(count, rows, cols);
   if (tiled) {
     args.arrived = (int*)at;
     args.partial = (float*)(at + NS_HEAD);
-    at += shared_bytes(tile);
-    used = shared_bytes(tile);
+    used = shared_bytes(plan);
+    at += used;
   }
   for (int i = 0; i < count; ++i) {
     if (!g[i] || !out[i] || (MUON && (!v[i]))) return DTF_ERR_BAD_ARG;
@@ -1006,10 +1096,10 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     at += s.xt;
     t.xt1 = at;
     at += s.xt;
-    t.a = at;
-    at += s.sq;
-    t.b = at;
-    at += s.sq;
+    for (char*& sq : t.sq) {
+      sq = at;
+      at += s.sq;
+    }
   }
   NsArgs parts = args, split = args;
   for (int i = 0; i < args.count; ++i) {
@@ -1019,16 +1109,22 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     parts.first[i + 1] = parts.first[i] + t.nparts;
     split.first[i + 1] = split.first[i] + (int)tiles;
   }
+  NsSet sets[2] = {{args, plan.tiles[0], false}, {args, plan.tiles[1], true}};
+  sets[0].args.count = sets[1].args.count = 0;
+  for (int i = 0; i < args.count; ++i) {
+    NsArgs& to = sets[plan.pairs && is_wide(args.t[i].rows, args.t[i].cols)].args;
+    to.t[to.count++] = args.t[i];
+  }
   switch (type) {
     case NS_F32:
-      return launch<float, MUON>(args, parts, split, thin, tile, steps, coef, eps, mo, stream);
+      return launch<float, MUON>(sets, parts, split, thin, steps, coef, factor, eps, mo, stream);
     case NS_BF16:
       if constexpr (!MUON)
-        return launch<dtf_bf16, false>(args, parts, split, thin, tile, steps, coef, eps, mo, stream);
+        return launch<dtf_bf16, false>(sets, parts, split, thin, steps, coef, factor, eps, mo, stream);
       break;
     default:
       if constexpr (!MUON)
-        return launch<_Float16, false>(args, parts, split, thin, tile, steps, coef, eps, mo, stream);
+        return launch<_Float16, false>(sets, parts, split, thin, steps, coef, factor, eps, mo, stream);
       break;
   }
   return DTF_ERR_BAD_ARG;
@@ -1046,7 +1142,7 @@ DTF_API long dtf_newton_schulz_workspace(int count, const int* rows, const int* 
     tiled = tiled || !is_thin(rows[i], cols[i]);
     total += sizes_of(rows[i], cols[i]).total;
   }
-  return total + (tiled ? shared_bytes(tile_of(count, rows, cols)) : 0);
+  return total + (tiled ? shared_bytes(plan_of(count, rows, cols)) : 0);
 }
 
 // out[i] = orthogonalised g[i], both [rows[i], cols[i]] contiguous of `type` (0 fp32, 1 bf16,

@@ -13,6 +13,11 @@ step's errors grow 485-fold, so the result, of norm about one, is off by at most
 value of the normalised input is one (rank one), and by that value times as much when it is
 smaller: ``_spectral_bound``. Those are worst cases of aligned errors; the root mean square of an
 element's error is held to the same bound times the root mean square of the result.
+Long matrices take two steps as one, X = B'(A') B X with A' = B A B: seven products. An error of d
+on A' changes B' by (|b| + 2 |c|) d < 9 d and one of d on A changes A' by a^2 d < 12 d, both times
+the square of the largest singular value; aligned worst cases may so reach a few times the bound
+of single steps when that value is near one, which errors of random sign do not: the same bound is
+asked of them.
 A 16-bit result adds its own rounding, eps / 2 per element."""
 import numpy as np
 import pytest
@@ -70,6 +75,8 @@ def _matrix(rows, cols, kind="gauss", seed=0):
     gen = torch.Generator().manual_seed(seed * 1009 + rows * 17 + cols)
     if kind == "gauss":
         return torch.randn(rows, cols, generator=gen)
+    if kind == "rank_one":
+        return torch.outer(torch.randn(rows, generator=gen), torch.randn(cols, generator=gen))
     rank = max(1, min(rows, cols) // 4)
     return torch.randn(rows, rank, generator=gen) @ torch.randn(rank, cols, generator=gen) * 1e-3
 
@@ -174,6 +181,41 @@ def test_many_large_matrices(hip, dtype):
     for g, out, again in zip(mats, outs, hip.newton_schulz(mats, steps=3)):
         assert torch.equal(out, again)
         _check(out, g, dtype, steps=3)
+
+
+# long matrices, which take steps in pairs: alone, beside others, with products on either tile
+LONG = [[(301, 7001)], [(7001, 129)], [(500, 8000), (40, 50), (333, 350), (8001, 300)],
+        [(1300, 1701), (1701, 1300), (1299, 1699)]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["gauss", "low_rank", "rank_one"])
+@pytest.mark.parametrize("shapes", LONG)
+def test_long_matrices(hip, shapes, kind):
+    mats = [_matrix(r, c, kind).cuda() for r, c in shapes]
+    for g, out in zip(mats, hip.newton_schulz(mats)):
+        _check(out, g, F32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7])
+def test_step_counts_of_long_matrices(hip, steps):
+    g = _matrix(129, 6000).cuda()
+    _check(hip.newton_schulz(g, steps=steps), g, F32, steps=steps)
+    h = g.t().contiguous().bfloat16()
+    _check(hip.newton_schulz(h, steps=steps), h, BF16, steps=steps)
+    # factors whose product the images cannot hold: 4.2 and 4 stay single steps
+    rows = [(4.2, -6.0, 2.4), (4.0, -2.85, 0.59), (2.0, -0.4, 0.035), (1.5, -0.1, 0.0)][:steps]
+    _check(hip.newton_schulz(g, steps=len(rows), coefficients=rows), g, F32, steps=len(rows),
+           coef=rows)
+
+
+@pytest.mark.gpu
+def test_wide_tiles_for_every_product(hip):
+    shapes = [(2047, 2049), (2001, 1999), (1999, 5000), (5001, 1987)]
+    mats = [_matrix(r, c).cuda() for r, c in shapes]
+    for g, out in zip(mats, hip.newton_schulz(mats, steps=2)):
+        _check(out, g, F32, steps=2)
 
 
 @pytest.mark.gpu
