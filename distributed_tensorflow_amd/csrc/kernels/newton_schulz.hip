@@ -47,10 +47,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 struct yes {
-  static constexpr bool value = true;
+  static constexpr int value = 1;
 };
 struct no {
-  static constexpr bool value = false;
+  static constexpr int value = 0;
 };
 
 enum { NS_F32 = 0, NS_BF16 = 1, NS_F16 = 2 };
@@ -498,7 +498,10 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArg
 
 // 64 x 64 tiles: four multiplying waves and four that issue the LDS-DMA requests, three K-tiles
 // ahead into four buffers -- the multiplying waves never wait at the address unit. Two workgroups
-// per CU. (Four waves that do both: 1024 x 1024 302 us instead of 186.)
+// per CU. (Four waves that do both: 1024 x 1024 302 us instead of 186.) A workgroup that has its CU to
+// itself takes 0.23 us per K-tile, the time the 16 KB of requests take: six and eight buffers, or
+// requests to registers and stores from there, were 10 to 20 % slower. Two on a CU are bound by
+// the LDS: 48 KB in and out per K-tile.
 template <typename E, int TO, bool MUON>
 __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, float ca, float cb,
                                               float cc, const NsMuon& mo) {
@@ -560,20 +563,33 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
     if (w.splits == 1) return;
   } else {
     f32x4 acc[NI][NI];
-    // one K-tile; FIRST: the accumulators start from zero
-    auto multiply = [&](int kt, auto first) {
-      constexpr bool FIRST = decltype(first)::value;
-      // K-tile kt has landed for every wave, and every wave is done with the buffer before it
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // fragments of two K-tiles: one is read while the other is multiplied
+    f16x8 ph[2][NI], pl[2][NI], qh[2][NI], ql[2][NI];
+    auto fetch = [&](int kt, auto odd) {
+      constexpr int S = decltype(odd)::value;
       const char* cur = smem + kt % NB * BUF_BYTES;
-      f16x8 ph[NI], pl[NI], qh[NI], ql[NI];
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int rp = wr * WT + i * 16 + frow, rq = wc * WT + i * 16 + frow;
-        ph[i] = *reinterpret_cast<const f16x8*>(cur + piece_off(rp, fq));
-        pl[i] = *reinterpret_cast<const f16x8*>(cur + piece_off(rp, 4 + fq));
-        qh[i] = *reinterpret_cast<const f16x8*>(cur + OP_BYTES + piece_off(rq, fq));
-        ql[i] = *reinterpret_cast<const f16x8*>(cur + OP_BYTES + piece_off(rq, 4 + fq));
+        ql[S][i] = *reinterpret_cast<const f16x8*>(cur + OP_BYTES + piece_off(rq, 4 + fq));
+        ph[S][i] = *reinterpret_cast<const f16x8*>(cur + piece_off(rp, fq));
+        qh[S][i] = *reinterpret_cast<const f16x8*>(cur + OP_BYTES + piece_off(rq, fq));
+        pl[S][i] = *reinterpret_cast<const f16x8*>(cur + piece_off(rp, 4 + fq));
+      }
+    };
+    // one K-tile; FIRST: the accumulators start from zero
+    auto multiply = [&](int kt, auto odd, auto first) {
+      constexpr int S = decltype(odd)::value;
+      constexpr bool FIRST = decltype(first)::value;
+      // this K-tile's fragments are here, so its buffer is free behind the barrier; the next
+      // K-tile has landed for every wave
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (kt + 1 < w.nkt) {
+        asm volatile("s_barrier" ::: "memory");
+        if constexpr (S == 0)
+          fetch(kt + 1, yes());
+        else
+          fetch(kt + 1, no());
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i)
@@ -581,15 +597,21 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
         for (int j = 0; j < NI; ++j) {
           // (operands swapped: a lane's four results lie along N)
           const f32x4 from = FIRST ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j];
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph[i], from, 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl[i], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph[i], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[S][j], ph[S][i], from, 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[S][j], pl[S][i], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[S][j], ph[S][i], acc[i][j], 0, 0, 0);
         }
     };
+    asm volatile("s_barrier" ::: "memory");       // K-tile 0 has landed
+    fetch(0, no());
+    static_assert(NS_CHAIN % 2 == 0, "fragment sets alternate");
     for (int base = 0; base < w.nkt; base += NS_CHAIN) {
-      multiply(base, yes());
-      const int end = base + NS_CHAIN < w.nkt ? base + NS_CHAIN : w.nkt;
-      for (int kt = base + 1; kt < end; ++kt) multiply(kt, no());
+      multiply(base, no(), yes());
+#pragma unroll
+      for (int k = 1; k < NS_CHAIN; k += 2) {
+        if (base + k < w.nkt) multiply(base + k, yes(), no());
+        if (k + 1 < NS_CHAIN && base + k + 1 < w.nkt) multiply(base + k + 1, no(), no());
+      }
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
