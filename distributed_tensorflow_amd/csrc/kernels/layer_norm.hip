@@ -112,17 +112,21 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layer_norm_kernel(
     if (gamma) load_part<V>(gamma, c, cols, gm[j]);
     if (beta) load_part<V>(beta, c, cols, bt[j]);
   }
-  // (L >= 256: one row per workgroup, so the loop count is the same for every wave that meets at
-  // the barriers; smaller groups never leave their wave. Requesting the next row before this one
-  // is worked on, as the backward kernel does, made the large cases 10-25 % slower: eight or more
+  // (Groups of several waves meet at barriers, so every group of a workgroup runs the same number
+  // of turns; one behind the last row works on zeros. Requesting the next row before this one is
+  // worked on, as the backward kernel does, made the large cases 10-25 % slower: eight or more
   // waves per SIMD cover the loads, and the registers cost some of them.)
-  for (long row = blockIdx.x * (long)GROUPS + group; row < rows; row += (long)gridDim.x * GROUPS) {
-    const T* xr = x + row * ldx;
+  for (long row0 = blockIdx.x * (long)GROUPS; row0 < rows; row0 += (long)gridDim.x * GROUPS) {
+    const long row = row0 + group;
+    const bool live = GROUPS == 1 || row < rows;
+    if (L <= 64 && !live) break;
+    const T* xr = x + (live ? row : 0) * ldx;
+    const int here = live ? cols : 0;
     float v[NV][V];
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      load_part<V>(xr, (lane + j * L) * V, cols, v[j]);
+      load_part<V>(xr, (lane + j * L) * V, here, v[j]);
 #pragma unroll
       for (int k = 0; k < V; ++k) s += v[j][k];
     }
@@ -149,6 +153,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layer_norm_kernel(
     const float fix = s * inv_n;
     const float var = __builtin_fmaf(-fix, fix, q * inv_n);
     const float rstd = 1.f / __builtin_sqrtf((var > 0.f ? var : 0.f * var) + eps);
+    if (!live) continue;
     T* yr = y + row * (long)cols;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -464,21 +469,21 @@ Plan plan_of(long cols, int v) {
 }
 
 // CALL(lanes, vectors per lane) of the plan
-#define LN_FOR_PLAN(PLAN, CALL)                                \
-  if ((PLAN).nv * V > LANE_ELEMS) {                                    \
-    CALL(1024, 16 / V);                                        \
-  } else {                                                     \
-    switch ((PLAN).lanes) {                                    \
-      case 4: CALL(4, LANE_ELEMS / V); break;                           \
-      case 8: CALL(8, LANE_ELEMS / V); break;                           \
-      case 16: CALL(16, LANE_ELEMS / V); break;                         \
-      case 32: CALL(32, LANE_ELEMS / V); break;                         \
-      case 64: CALL(64, LANE_ELEMS / V); break;                         \
-      case 128: CALL(128, LANE_ELEMS / V); break;                       \
-      case 256: CALL(256, LANE_ELEMS / V); break;                       \
-      case 512: CALL(512, LANE_ELEMS / V); break;                       \
-      default: CALL(1024, LANE_ELEMS / V); break;                       \
-    }                                                          \
+#define LN_FOR_PLAN(PLAN, CALL)                                       \
+  if ((PLAN).nv * V > LANE_ELEMS) {                                   \
+    CALL(1024, 16 / V);                                               \
+  } else {                                                            \
+    switch ((PLAN).lanes) {                                           \
+      case 4: CALL(4, LANE_ELEMS / V); break;                         \
+      case 8: CALL(8, LANE_ELEMS / V); break;                         \
+      case 16: CALL(16, LANE_ELEMS / V); break;                       \
+      case 32: CALL(32, LANE_ELEMS / V); break;                       \
+      case 64: CALL(64, LANE_ELEMS / V); break;                       \
+      case 128: CALL(128, LANE_ELEMS / V); break;                     \
+      case 256: CALL(256, LANE_ELEMS / V); break;                     \
+      case 512: CALL(512, LANE_ELEMS / V); break;                     \
+      default: CALL(1024, LANE_ELEMS / V); break;                     \
+    }                                                                 \
   }
 
 long min_l(long a, long b) { return a < b ? a : b; }
