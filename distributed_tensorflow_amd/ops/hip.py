@@ -11,6 +11,7 @@ missing, importing this module's users fails loudly rather than falling back to 
 """
 from __future__ import annotations
 
+import bisect
 import contextlib
 import ctypes
 import os
@@ -1404,7 +1405,7 @@ def multi_muon(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         raise HipKernelError("multi_muon: epsilon must not be negative, got %r" % (epsilon,))
     coef = _ns_coefficients(coefficients, steps, what)
     work = []
-    spans = []
+    span = lambda t: (t.data_ptr(), t.data_ptr() + 4 * t.numel())             # noqa: E731
     for i, (p, g, m) in enumerate(zip(params, grads, moments)):
         for t in (p, g, m):
             if t.dtype != torch.float32 or t.device.type != "cuda" or t.device != params[0].device \
@@ -1415,18 +1416,20 @@ def multi_muon(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
             raise HipKernelError("multi_muon: params and moments must be contiguous")
         if p.numel() == 0:
             continue
-        g = g if g.is_contiguous() else g.contiguous()
-        spans += [(t.data_ptr(), t.data_ptr() + 4 * t.numel(), writes)
-                  for t, writes in ((p, True), (m, True), (g, False))]
         scale = float(scales[i]) if scales is not None else muon_scale(*p.shape[-2:])
-        work += [(a, b, c, scale) for a, b, c in
-                 (zip(p, g, m) if p.dim() == 3 else ((p, g, m),))]
-    written = read = 0                # how far the memory of the ones before reaches
-    for lo, hi, writes in sorted(spans):
-        if lo < written or writes and lo < read:
-            raise HipKernelError("multi_muon: params and moments overlap in memory, or a gradient "
-                                 "lies in one of them")
-        written, read = (max(written, hi), read) if writes else (written, max(read, hi))
+        work.append((p, g if g.is_contiguous() else g.contiguous(), m, scale))
+    written = sorted(span(t) for p, _, m, _ in work for t in (p, m))
+    if any(a[1] > b[0] for a, b in zip(written, written[1:])):
+        raise HipKernelError("multi_muon: params and moments overlap in memory")
+    # a gradient that lies in what is updated (of w w / 2 it is w itself) is read from a copy
+    starts = [lo for lo, _ in written]
+    for i, (p, g, m, scale) in enumerate(work):
+        lo, hi = span(g)
+        at = bisect.bisect_left(starts, hi)          # spans from here on start behind g
+        if at and written[at - 1][1] > lo:
+            work[i] = (p, g.clone(), m, scale)
+    work = [(a, b, c, scale) for p, g, m, scale in work
+            for a, b, c in (zip(p, g, m) if p.dim() == 3 else ((p, g, m),))]
     if lr_dev is not None and work and lr_dev.device != work[0][0].device:
         raise HipKernelError("multi_muon: lr is on another device")
     c = ctypes

@@ -801,10 +801,18 @@ def _optim_launch(ctx, rule, hyper, var_ops, slot_ops_list, power_ops, grads, lr
     if ps and rule == "muon":
         from .ref_kernels import muon_rule
         h, coef, _ = muon_rule(hyper, ps[0].shape)
-        hip.multi_muon(ps, [g.view(p.shape) for p, g in zip(ps, gs)], s0,
-                       h["lr"] if lr is None else lr, h["momentum"], bool(h["nesterov"]),
-                       h["weight_decay"], [muon_rule(hyper, p.shape)[2] for p in ps],
-                       int(h["steps"]), coef, h["epsilon"])
+        left = list(zip(ps, gs, s0))
+        while left:                        # (a variable that is updated twice: one after the other)
+            first = {}
+            for item in left:
+                first.setdefault(item[0].data_ptr(), item)
+            left = [item for item in left if first[item[0].data_ptr()] is not item]
+            now = list(first.values())
+            hip.multi_muon([p for p, _, _ in now], [g.view(p.shape) for p, g, _ in now],
+                           [v for _, _, v in now], h["lr"] if lr is None else lr, h["momentum"],
+                           bool(h["nesterov"]), h["weight_decay"],
+                           [muon_rule(hyper, p.shape)[2] for p, _, _ in now], int(h["steps"]),
+                           coef, h["epsilon"])
     elif ps:
         hip.multi_optim(rule, ps, gs, s0, s1, hyper, powers, lr=lr)
     return rest

@@ -274,3 +274,33 @@ def test_gpu_newton_schulz_op():
     with tf.Session(config=tf.ConfigProto(device="cuda:0")) as sess:
         got = sess.run(tf.newton_schulz(x), {x: v})
     np.testing.assert_allclose(got, _ns64(v), rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("fusion", [True, False])
+def test_gradients_that_are_the_weights_and_weights_updated_twice(device, fusion):
+    """The gradient of w w / 2 is w itself: it is read before w is written. A matrix given twice
+    is updated twice. (Tolerance: the rule's result is off by at most 2e-3 in the spectral norm,
+    times the rate; the momentum of the second update adds its own.)"""
+    rng = np.random.RandomState(5)
+    values = [rng.randn(*s).astype(np.float32) for s in ((70, 90), (12, 10), (90, 33), (20, 24))]
+    for twice in (False, True):
+        with tf.Graph().as_default():
+            ws = [tf.Variable(tf.constant(v), name="w%d" % i) for i, v in enumerate(values)]
+            loss = tf.add(tf.add(tf.nn.l2_loss(ws[0]), tf.nn.l2_loss(ws[1])),
+                          tf.add(tf.nn.l2_loss(ws[2]), tf.nn.l2_loss(ws[3])))
+            opt = tf.train.MuonOptimizer(0.05)
+            gv = opt.compute_gradients(loss)
+            train = opt.apply_gradients(gv + [(tf.identity(g), v) for g, v in gv[:2]]
+                                        if twice else gv)
+            with tf.Session(config=tf.ConfigProto(device=device, graph_fusion=fusion)) as sess:
+                sess.run(tf.global_variables_initializer())
+                sess.run(train)
+                got = sess.run(ws)
+        for i, (w, g) in enumerate(zip(values, got)):
+            s = max(1.0, w.shape[1] / w.shape[0]) ** 0.5
+            if not (twice and i < 2):
+                assert np.abs(g - (w - 0.05 * s * _ns64(w))).max() <= 0.05 * s * 2e-3
+            elif fusion or device == "cpu":
+                # both gradients are the weight's value before the step
+                assert np.abs(g - (w - 0.1 * s * _ns64(w))).max() <= 0.1 * s * 2e-3
