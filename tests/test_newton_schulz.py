@@ -132,6 +132,29 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
             call()
 
 
+def test_product_kernels_use_no_scratch(tmp_path):
+    """The products wait for their LDS-DMA requests with counted ``s_waitcnt vmcnt(N)``: a spilled
+    register's loads and stores would be counted with them."""
+    import os
+    import re
+    import shutil
+    import subprocess
+    from distributed_tensorflow_amd.ops import hip
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("hipcc not installed")
+    kernels = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(hip.__file__))), "csrc",
+                           "kernels")
+    asm = str(tmp_path / "k.s")
+    subprocess.run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only",
+                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I" + kernels,
+                    "-o", asm, os.path.join(kernels, "newton_schulz.hip")], check=True, timeout=600)
+    sizes = [int(m.group(2)) for m in re.finditer(r"^(_Z\w+):.*?; ScratchSize: (\d+)",
+                                                  open(asm).read(), re.S | re.M)
+             if "ns_product_kernel" in m.group(1)]
+    assert len(sizes) >= 10 and not any(sizes), sizes
+
+
 # ---------------------------------------------------------------------------------------
 # kernels
 # ---------------------------------------------------------------------------------------
