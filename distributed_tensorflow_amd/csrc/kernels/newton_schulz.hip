@@ -23,7 +23,8 @@
 // operands are K-contiguous. Long matrices take two steps as one (step_pairs), which leaves out
 // every other pair of products with X. The matrices of one call (up to NS_MAX_MATS, any shapes)
 // share each launch: two, and three per step, whatever the count; long ones may have a sequence of
-// their own, and matrices of up to 64 rows or columns have (newton_schulz_thin.h).
+// their own, and matrices of up to 64 rows or columns have (newton_schulz_thin.h). Calls of nothing
+// larger than 128 x 2048 take one or two steps in a launch (newton_schulz_mid.h).
 //
 // Layout. "Split rows": row r of K elements takes 4 bytes per element, in chunks of 32 elements:
 // 32 hi halves (64 bytes), then 32 lo halves. A chunk is 128 bytes, so a K-tile of 32 elements has
@@ -72,6 +73,7 @@ struct NsMat {
   float scale;         // Muon: s
   double* gram;        // thin matrices: [slabs][lower 16 x 16 tiles][256]
   int slabs, slab_cols;
+  char* a_parts[2];    // up to 128 x 2048: the slabs' parts of A, read and written in turn
 };
 struct NsArgs {
   NsMat t[NS_MAX_MATS];
@@ -755,16 +757,25 @@ __global__ __launch_bounds__(512, T == 64 ? 4 : 2) void ns_product_kernel(
 }
 
 #include "newton_schulz_thin.h"
+#include "newton_schulz_mid.h"
 
 // ---- host ------------------------------------------------------------------------------------
 long up(long v, long to) { return (v + to - 1) / to * to; }
 
 bool is_thin(long rows, long cols) { return (rows < cols ? rows : cols) <= THIN_M; }
 
+// (up to 128 x 2048, as newton_schulz_mid.h says)
+bool is_mid(long rows, long cols) {
+  const long m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return !is_thin(rows, cols) && m <= MID_M && n <= MID_N;
+}
+long mid_slabs(long n) { return (n + MID_SLAB - 1) / MID_SLAB; }
+
 struct NsSizes {
   long m, n, km, kn, parts;
   long slabs, slab_cols;          // thin matrices
   long x, xt, sq;                 // bytes of one image
+  long a_parts;                   // of the slabs' parts
   long total;
 };
 NsSizes sizes_of(long rows, long cols) {
@@ -785,7 +796,8 @@ NsSizes sizes_of(long rows, long cols) {
   s.x = up(s.m * pitch_of((int)s.kn), 256);
   s.xt = up(s.n * pitch_of((int)s.km), 256);
   s.sq = up(s.m * pitch_of((int)s.km), 256);
-  s.total = up(8 * s.parts, 256) + s.x + 2 * s.xt + 3 * s.sq;
+  s.a_parts = is_mid(rows, cols) ? mid_slabs(s.n) * MID_PART : 0;
+  s.total = up(8 * s.parts, 256) + s.x + 2 * s.xt + 3 * s.sq + 2 * s.a_parts;
   return s;
 }
 
@@ -1024,6 +1036,41 @@ int launch_steps(const NsSet& set, int steps, const float* coef, const double* f
   return DTF_OK;
 }
 
+// The whole call in launches of one or two steps (newton_schulz_mid.h)
+template <int KT, typename E, bool MUON>
+int launch_mid(const NsArgs& args, int steps, const float* coef, const double* factor, float eps,
+               const NsMuon& mo, hipStream_t stream) {
+  constexpr int LDS = 2 * MID_MAT;
+  static DtfPerDeviceOnce once;
+  dtf_once_per_device(once, [&] {
+    allow_lds(ns_mid_kernel<KT, E, MID_FIRST, MUON>, LDS);
+    allow_lds(ns_mid_kernel<KT, float, MID_STEP, false>, LDS);
+    allow_lds(ns_mid_kernel<KT, E, MID_LAST, MUON>, LDS);
+  });
+  MidArgs now = {};
+  now.count = args.count;
+  for (int i = 0; i < args.count; ++i) {
+    now.t[i] = args.t[i];
+    now.first[i + 1] = now.first[i] + (int)mid_slabs(args.t[i].n);
+  }
+  const dim3 grid(now.first[now.count]), block(MID_THREADS);
+  hipLaunchKernelGGL((ns_mid_kernel<KT, E, MID_FIRST, MUON>), grid, block, LDS, stream, now, eps, mo);
+  for (int k = 0; k < steps;) {
+    now.pair = step_pairs(k, steps, factor);
+    ++now.turn;
+    for (int i = 0; i < 3 + 3 * now.pair; ++i) now.c[i] = coef[3 * k + i];
+    k += 1 + now.pair;
+    if (k < steps)
+      hipLaunchKernelGGL((ns_mid_kernel<KT, float, MID_STEP, false>), grid, block, LDS, stream, now,
+                         eps, mo);
+    else
+      hipLaunchKernelGGL((ns_mid_kernel<KT, E, MID_LAST, MUON>), grid, block, LDS, stream, now, eps,
+                         mo);
+  }
+  DTF_LAUNCH_CHECK();
+  return DTF_OK;
+}
+
 // head of the workspace: arrival counts, then the partial tiles of one split product
 constexpr long NS_HEAD = 4L * NS_SLOTS;
 long shared_bytes(const NsPlan& plan) {
@@ -1046,6 +1093,15 @@ int launch(const NsSet (&sets)[2], const NsArgs& parts, const NsArgs& split, con
   if (n == 0) return DTF_OK;
   hipLaunchKernelGGL((ns_norm_kernel<E, MUON>), dim3(parts.first[n]), dim3(256), 0, stream, parts,
                      mo);
+  DTF_LAUNCH_CHECK();
+  bool mid = true;
+  int m = 0;
+  for (int i = 0; i < n; ++i) {
+    mid = mid && is_mid(parts.t[i].rows, parts.t[i].cols);
+    m = parts.t[i].m > m ? parts.t[i].m : m;
+  }
+  if (mid && m <= 96) return launch_mid<3, E, MUON>(parts, steps, coef, factor, eps, mo, stream);
+  if (mid) return launch_mid<4, E, MUON>(parts, steps, coef, factor, eps, mo, stream);
   hipLaunchKernelGGL((ns_split_kernel<E, MUON>), dim3(split.first[n]), dim3(256), 0, stream, split,
                      eps, mo);
   DTF_LAUNCH_CHECK();
@@ -1121,6 +1177,10 @@ int run(int count, const void* const* g, void* const* out, float* const* v, cons
     for (char*& sq : t.sq) {
       sq = at;
       at += s.sq;
+    }
+    for (char*& a : t.a_parts) {
+      a = at;
+      at += s.a_parts;
     }
   }
   NsArgs parts = args, split = args;

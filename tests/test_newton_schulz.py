@@ -206,6 +206,88 @@ def test_many_large_matrices(hip, dtype):
         _check(out, g, dtype, steps=3)
 
 
+# up to 128 x 2048, which take one or two steps in a launch, and the sizes next to them
+MID = [[(65, 65)], [(128, 128)], [(129, 128)], [(96, 97)], [(97, 96)], [(128, 2048)], [(2048, 128)],
+       [(2049, 128)], [(66, 2047)], [(2000, 65)], [(100, 784), (784, 100), (10, 100), (128, 1000),
+                                                   (65, 2048), (333, 81), (120, 120)] * 2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("kind", ["gauss", "low_rank", "rank_one"])
+@pytest.mark.parametrize("shapes", MID)
+def test_mid_matrices(hip, shapes, kind, dtype):
+    mats = [_matrix(r, c, kind, seed=i).to(dtype).cuda() for i, (r, c) in enumerate(shapes)]
+    outs = hip.newton_schulz(mats)
+    for g, out, again in zip(mats, outs, hip.newton_schulz(mats)):
+        assert torch.equal(out, again)
+        _check(out, g, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 6])
+def test_step_counts_of_mid_matrices(hip, steps):
+    for g in (_matrix(100, 300).cuda(), _matrix(300, 90).cuda()):
+        _check(hip.newton_schulz(g, steps=steps), g, F32, steps=steps)
+    # factors whose product the images cannot hold: 4.2 and 4 stay single steps
+    rows = [(4.2, -6.0, 2.4), (4.0, -2.85, 0.59), (2.0, -0.4, 0.035), (1.5, -0.1, 0.0)][:steps]
+    _check(hip.newton_schulz(g, steps=len(rows), coefficients=rows), g, F32, steps=len(rows),
+           coef=rows)
+
+
+@pytest.mark.gpu
+def test_special_values_of_mid_matrices(hip):
+    mats = [torch.zeros(100, 200), _matrix(100, 200), _matrix(200, 100) * 1e-25, torch.zeros(70, 70),
+            _matrix(90, 90) * 1e25]
+    mats = [m.cuda() for m in mats]
+    clean = hip.newton_schulz(mats, epsilon=0.0)
+    for i in (0, 3):
+        assert torch.isnan(clean[i]).all()                    # 0 / 0, in its own matrix alone
+    for i in (1, 2, 4):
+        _check(clean[i], mats[i], F32, eps=0.0)
+    zeros = hip.newton_schulz(mats)
+    assert torch.equal(zeros[0], mats[0]) and torch.equal(zeros[3], mats[3])
+    for bad in (float("nan"), float("inf")):
+        mats[1][7, 9] = bad
+        out = hip.newton_schulz(mats, epsilon=0.0)
+        assert torch.isnan(out[1]).any()
+        for i in (2, 4):
+            assert torch.equal(out[i], clean[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_of_mid_matrices_on_a_stream_and_replayed(hip, nesterov):
+    shapes = [(784, 100), (100, 10), (66, 70), (128, 2048), (1500, 97)]
+    gs = [_matrix(*s).cuda() for s in shapes]
+    ws, vs = ([_matrix(*s, seed=k).cuda() for s in shapes] for k in (1, 2))
+    w0, v0 = [w.clone() for w in ws], [v.clone() for v in vs]
+    want = [muon_exact(w, g, v, 0.05, nesterov=nesterov, decay=0.1) for w, g, v in zip(ws, gs, vs)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        hip.multi_muon(ws, gs, vs, 0.05, nesterov=nesterov, weight_decay=0.1)
+    side.synchronize()
+    for w, v, old, (ew, ev, u) in zip(ws, vs, w0, want):
+        s = max(1.0, w.shape[1] / w.shape[0]) ** 0.5
+        tol = 0.05 * s * _spectral_bound(u) + 4 * 2.0 ** -24 * (old.abs().max().item() + 0.05 * s)
+        assert (w.double().cpu() - ew).abs().max().item() <= tol
+        # the product, the sum and 0.95 itself round
+        assert (v.double().cpu() - ev).abs().max().item() <= 4 * 2.0 ** -24 * ev.abs().max().item() * 2
+    a, b = [w.clone() for w in w0], [v.clone() for v in v0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hip.multi_muon(a, gs, b, 0.05, nesterov=nesterov, weight_decay=0.1)
+    for x, y in zip(a + b, w0 + v0):
+        x.copy_(y)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(a + b, ws + vs):
+            assert torch.equal(x, y)
+        hip.multi_muon(ws, gs, vs, 0.05, nesterov=nesterov, weight_decay=0.1)
+
+
 # long matrices, which take steps in pairs: alone, beside others, with products on either tile
 LONG = [[(301, 7001)], [(7001, 129)], [(500, 8000), (40, 50), (333, 350), (8001, 300)],
         [(1300, 1701), (1701, 1300), (1299, 1699)]]
