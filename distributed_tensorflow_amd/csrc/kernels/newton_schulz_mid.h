@@ -6,13 +6,12 @@
 // columns of X in place of one: every workgroup adds up A = X X^T from the slabs' parts, goes
 // through the polynomials of one step or of a pair of them by itself, multiplies its own slab, X =
 // P X, and leaves the slab's part of the next A. Five steps are five launches with the norm and the
-// first A: 128 x 128 63 us (tiled 89), 784 x 100 80 (109), 128 x 2048 97 (115), sixteen 128 x 2048 147
-// (168). A slab costs 0.4 us a launch to add up, so rows longer than 2048 are left to the tiles, and
+// first A: 128 x 128 63 us (tiled 89), 784 x 100 77 (109), 128 x 2048 93 (115), sixteen 128 x 2048 143
+// (166). A slab costs 0.7 us a launch to add up, so rows longer than 2048 are left to the tiles, and
 // so are calls with a larger matrix, whose launches take these along.
 //
 // What bounds it: 2 to 3 us a product on one CU, of which the matrix instructions are 1.3 and the
-// LDS reads as much; the rest is rounding to pairs and two barriers. (Pairs of values converted
-// in one instruction and loops over K unrolled: 784 x 100 92 -> 82 us.)
+// LDS reads as much; the rest is rounding to pairs and two barriers.
 //
 // One buffer holds B, the other A, then C = B A, A' = C B, B' = q'(A'), and P = B' B goes where B
 // was. The products are commuting polynomials of one A, symmetric up to rounding, and are read by
@@ -181,14 +180,24 @@ __global__ __launch_bounds__(MID_THREADS) void ns_mid_kernel(MidArgs args, float
     u32x4 held[8];
     mid_request(t.xt0 + n0 * xt_pitch, width, t.km / 32, held);
     // A: the parts in slab order
-    const f32x4* part = reinterpret_cast<const f32x4*>(t.a_parts[(args.turn + 1) & 1]) + threadIdx.x;
-    each([&](int i, int j, int, int) { acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f}; });
+    const __amdgpu_buffer_rsrc_t parts = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)t.a_parts[(args.turn + 1) & 1], 0, slabs * MID_PART, 0x00020000);
+    // (16 x 16 blocks behind the last row or column are not fetched: an offset out of range)
+    int at[4][2];
+    each([&](int i, int j, int, int) {
+      acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      at[i][j] = wm + 16 * i < t.m && wn + 16 * j < t.m
+                     ? ((i * 2 + j) * MID_THREADS + (int)threadIdx.x) * 16
+                     : 0x40000000;
+    });
 #pragma unroll 4
     for (int s = 0; s < slabs; ++s) {
       f32x4 v[4][2];
-      each([&](int i, int j, int, int) { v[i][j] = part[(i * 2 + j) * MID_THREADS]; });
+      each([&](int i, int j, int, int) {
+        v[i][j] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, at[i][j], s * MID_PART, 0));
+      });
       each([&](int i, int j, int, int) { acc[i][j] += v[i][j]; });
-      part += MID_PART / 16;
     }
     each([&](int i, int j, int m, int n) {
       mid_put(U, m, n, acc[i][j] * (AB_SCALE / (X_SCALE * X_SCALE)));
@@ -291,6 +300,8 @@ __global__ __launch_bounds__(MID_THREADS) void ns_mid_kernel(MidArgs args, float
     mid_product<4>(U, U, wm, wn, acc);
     f32x4* part = reinterpret_cast<f32x4*>(t.a_parts[args.turn & 1] + (long)slab * MID_PART) +
                   threadIdx.x;
-    each([&](int i, int j, int, int) { part[(i * 2 + j) * MID_THREADS] = acc[i][j]; });
+    each([&](int i, int j, int, int) {
+      if (wm + 16 * i < t.m && wn + 16 * j < t.m) part[(i * 2 + j) * MID_THREADS] = acc[i][j];
+    });
   }
 }
