@@ -46,6 +46,8 @@ constexpr double X_LIMIT = 3.5, AB_LIMIT = 15.0;   // times the scales: below fp
 typedef __attribute__((address_space(3))) void lds_void;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 struct yes {
   static constexpr int value = 1;
@@ -104,6 +106,17 @@ __device__ __forceinline__ unsigned split_pack(float v) {
   const _Float16 lo = (_Float16)(v - (float)hi);
   return (unsigned)__builtin_bit_cast(unsigned short, hi) |
          (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
+}
+
+// four elements' hi halves and lo halves (two conversions in an instruction)
+__device__ __forceinline__ void split4(f32x4 v, uint2& hi, uint2& lo) {
+  const f16x2 h0 = __builtin_convertvector(f32x2{v[0], v[1]}, f16x2);
+  const f16x2 h1 = __builtin_convertvector(f32x2{v[2], v[3]}, f16x2);
+  const f32x2 r0 = {v[0] - (float)h0[0], v[1] - (float)h0[1]};
+  const f32x2 r1 = {v[2] - (float)h1[0], v[3] - (float)h1[1]};
+  hi = uint2{__builtin_bit_cast(unsigned, h0), __builtin_bit_cast(unsigned, h1)};
+  lo = uint2{__builtin_bit_cast(unsigned, __builtin_convertvector(r0, f16x2)),
+             __builtin_bit_cast(unsigned, __builtin_convertvector(r1, f16x2))};
 }
 
 // eight packed elements -> 16 bytes of hi, 16 bytes of lo
@@ -464,14 +477,18 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArg
                                                  m == n + r ? ca * AB_SCALE : 0.f));
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) pk[i][j][r] = m < M && n + r < N ? split_pack(v[r]) : 0u;
+        for (int r = 0; r < 4; ++r) v[r] = m < M && n + r < N ? v[r] : 0.f;
+        uint2 hi, lo;
+        split4(v, hi, lo);
+        unsigned* p = pk[i][j];
+        p[0] = (hi.x & 0xffffu) | lo.x << 16;
+        p[1] = hi.x >> 16 | (lo.x & 0xffff0000u);
+        p[2] = (hi.y & 0xffffu) | lo.y << 16;
+        p[3] = hi.y >> 16 | (lo.y & 0xffff0000u);
         if (m < M && (n & ~31) < N) {
           char* dst = direct + m * d_pitch + split_off(n);
-          const unsigned* p = pk[i][j];
-          *reinterpret_cast<uint2*>(dst) = uint2{(p[0] & 0xffffu) | p[1] << 16,
-                                                 (p[2] & 0xffffu) | p[3] << 16};
-          *reinterpret_cast<uint2*>(dst + 64) = uint2{p[0] >> 16 | (p[1] & 0xffff0000u),
-                                                      p[2] >> 16 | (p[3] & 0xffff0000u)};
+          *reinterpret_cast<uint2*>(dst) = hi;
+          *reinterpret_cast<uint2*>(dst + 64) = lo;
         }
       }
     if (SYM && row_block == col_block) continue;   // a diagonal block is its own mirror image

@@ -74,19 +74,9 @@ __device__ __forceinline__ int mid_off(int m, int n, int lo) {
   return (n >> 5) * MID_KT + piece_off(m, 4 * lo + ((n & 31) >> 3)) + (n & 7) * 2;
 }
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void mid_put(char* to, int m, int n, f32x4 v) {
   uint2 hi, lo;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {                  // (two conversions in an instruction)
-    const f32x2 x = {v[2 * r], v[2 * r + 1]};
-    const f16x2 h = __builtin_convertvector(x, f16x2);
-    const f32x2 rest = {x[0] - (float)h[0], x[1] - (float)h[1]};
-    const f16x2 l = __builtin_convertvector(rest, f16x2);
-    (r ? hi.y : hi.x) = __builtin_bit_cast(unsigned, h);
-    (r ? lo.y : lo.x) = __builtin_bit_cast(unsigned, l);
-  }
+  split4(v, hi, lo);
   *reinterpret_cast<uint2*>(to + mid_off(m, n, 0)) = hi;
   *reinterpret_cast<uint2*>(to + mid_off(m, n, 1)) = lo;
 }
