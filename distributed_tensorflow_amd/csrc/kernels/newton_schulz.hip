@@ -26,11 +26,12 @@
 // their own, and matrices of up to 64 rows or columns have (newton_schulz_thin.h). Calls of nothing
 // larger than 128 x 2048 take one or two steps in a launch (newton_schulz_mid.h).
 //
-// Layout. "Split rows": row r of K elements takes 4 bytes per element, in chunks of 32 elements:
-// 32 hi halves (64 bytes), then 32 lo halves. A chunk is 128 bytes, so a K-tile of 32 elements has
-// the LDS image of a 64-element bf16 K-tile (16-byte pieces, XOR-swizzled by row) and lands there
-// by 16-byte LDS-DMA. Rows are padded with zeros to whole chunks; edge tiles read the last row
-// again instead of rows that are not there.
+// Layout. An image of a matrix is a row of K-tiles of 32 columns; in a K-tile every row has 128
+// bytes: 32 hi halves, then 32 lo halves. So the rows of a K-tile that a workgroup wants lie in one
+// piece (with whole rows one behind the other, 4 K bytes apart, 1500 x 1500 took 408 us instead of
+// 391, 8192 x 4096 5.42 ms instead of 5.39), have the LDS image of a 64-element bf16 K-tile (16-byte
+// pieces, XOR-swizzled by row) and land there by 16-byte LDS-DMA. Columns are padded with zeros to
+// whole K-tiles; edge tiles read the last row again instead of rows that are not there.
 #include "elem.h"
 
 namespace {
@@ -64,13 +65,13 @@ struct NsMat {
   void* out;           // [rows, cols]; Muon: the weight
   float* v;            // Muon: momentum
   double* parts;       // [nparts] partial sums of squares
-  char* x;             // split rows [m][kn]
-  char* xt0;           // split rows [n][km]: read by even steps
+  char* x;             // image of [m][kn]
+  char* xt0;           // image of [n][km]: read by even steps
   char* xt1;           //                     ... by odd ones
-  char* sq[3];         // split rows [m][km]: A, B and products of them
+  char* sq[3];         // image of [m][km]: A, B and products of them
   int rows, cols;
   int m, n;
-  int km, kn;          // m, n rounded up to whole chunks
+  int km, kn;          // m, n rounded up to whole K-tiles
   int nparts;
   float scale;         // Muon: s
   double* gram;        // thin matrices: [slabs][lower 16 x 16 tiles][256]
@@ -131,11 +132,11 @@ __device__ __forceinline__ void store_split8(char* chunk_hi, const unsigned* p) 
   *reinterpret_cast<u32x4*>(chunk_hi + 64) = lo;
 }
 
-// byte offset of element c in a split row (its hi half; the lo half is 64 bytes further)
-__device__ __forceinline__ long split_off(int c) { return (long)(c >> 5) * 128 + (c & 31) * 2; }
-
-// (padding the pitch off the powers of two made the large products 1 to 9 % slower)
-__host__ __device__ __forceinline__ long pitch_of(int k) { return 4L * k; }
+// byte offset of element c of row r in an image of `rows` rows (its hi half; the lo half is 64
+// bytes further)
+__device__ __forceinline__ long image_off(int rows, int r, int c) {
+  return ((long)(c >> 5) * rows + r) * 128 + (c & 31) * 2;
+}
 
 // ---- momentum and sum of squares -------------------------------------------------------------
 // Squares are summed in 64 bits: gradients of 1e-20 or 1e+25 have squares fp32 does not hold.
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs args, NsMuon mo) {
     for (int i = threadIdx.x; i < NS_SLOTS; i += 256) args.arrived[i] = 0;
 }
 
-// ---- X and its transpose in split rows -------------------------------------------------------
+// ---- X and its transpose as images -----------------------------------------------------------
 // One 64 x 64 tile of G per workgroup: its rows go to one of the two orders as they are, its
 // columns through LDS to the other.
 template <typename E, bool MUON>
@@ -216,8 +217,6 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, float eps, N
   const bool tall = t.rows > t.cols;
   char* direct = tall ? t.xt0 : t.x;               // rows of `cols` elements
   char* turned = tall ? t.x : t.xt0;               // rows of `rows` elements
-  const long direct_pitch = pitch_of(tall ? t.km : t.kn);
-  const long turned_pitch = pitch_of(tall ? t.kn : t.km);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int rl = (threadIdx.x >> 3) + 32 * h, r = r0 + rl;
@@ -229,7 +228,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, float eps, N
       tr[(c8 + k) * 65 + rl] = p[k];
     }
     // (a chunk that starts inside the row belongs to it as a whole)
-    if (r < t.rows && (c & ~31) < t.cols) store_split8(direct + r * direct_pitch + split_off(c), p);
+    if (r < t.rows && (c & ~31) < t.cols) store_split8(direct + image_off(t.rows, r, c), p);
   }
   __syncthreads();
 #pragma unroll
@@ -239,7 +238,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, float eps, N
       unsigned p[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) p[k] = tr[cl * 65 + c8 + k];
-      store_split8(turned + (c0 + cl) * turned_pitch + split_off(r0 + c8), p);
+      store_split8(turned + image_off(t.cols, c0 + cl, r0 + c8), p);
     }
   }
 }
@@ -247,6 +246,12 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsArgs args, float eps, N
 // ---- the products ----------------------------------------------------------------------------
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const char* base) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0xffffffff, 0x00020000);
+}
+
+// rows r0 and on of K-tile kt
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const char* image, int rows, int r0,
+                                                            int kt) {
+  return rows_rsrc(image + ((long)kt * rows + r0) * 128);
 }
 
 // Workgroups that share a K range of kt K-tiles when `most` are offered. Parts go through memory
@@ -266,7 +271,7 @@ __device__ __forceinline__ int piece_off(int row, int kc) {
   return row * 128 + ((kc ^ ((row >> 1) & 7)) << 4);
 }
 
-// One BM x BN tile of P Q^T, P [M][K] and Q [N][K] in split rows. TO_A (X X^T), TO_B (a I + b A +
+// One BM x BN tile of P Q^T, images of P [M][K] and Q [N][K]. TO_A (X X^T), TO_B (a I + b A +
 // c A A) and TO_S (a product of polynomials of one A): symmetric results (M = N, tiles on and
 // below the diagonal), written to both places; TO_X: written in both orders; TO_OUT: the caller's
 // type.
@@ -451,7 +456,6 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArg
   if (SYM && row_block < col_block) return;
   char* direct = SYM ? t.sq[args.to] : t.x;                            // rows along M
   char* turned = TO == TO_X ? ((step & 1) ? t.xt0 : t.xt1) : direct;   // rows along N
-  const long d_pitch = pitch_of(TO == TO_X ? t.kn : t.km), t_pitch = pitch_of(t.km);
 #pragma unroll
   for (int h = 0; h < NM / 2; ++h) {
     // packed (hi | lo << 16) results; zero behind the last row and column
@@ -466,8 +470,7 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArg
         if (TO == TO_X || TO == TO_S) v *= 1.f / AB_SCALE;
         if (TO == TO_B) {
           // (any address inside for the elements that are not there: they become zeros below)
-          const char* src = t.sq[args.p] + (m < M ? m : 0) * t_pitch +
-                            split_off((n & ~31) < N ? n : 0);
+          const char* src = t.sq[args.p] + image_off(M, m < M ? m : 0, (n & ~31) < N ? n : 0);
           const f16x4 ah = *reinterpret_cast<const f16x4*>(src);
           const f16x4 al = *reinterpret_cast<const f16x4*>(src + 64);
 #pragma unroll
@@ -486,7 +489,7 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArg
         p[2] = (hi.y & 0xffffu) | lo.y << 16;
         p[3] = hi.y >> 16 | (lo.y & 0xffff0000u);
         if (m < M && (n & ~31) < N) {
-          char* dst = direct + m * d_pitch + split_off(n);
+          char* dst = direct + image_off(M, m, n);
           *reinterpret_cast<uint2*>(dst) = hi;
           *reinterpret_cast<uint2*>(dst + 64) = lo;
         }
@@ -509,7 +512,7 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArg
       const u32x4* src = reinterpret_cast<const u32x4*>(strip + nl * 36 + (lane & 3) * 8);
       *reinterpret_cast<u32x4*>(p) = src[0];
       *reinterpret_cast<u32x4*>(p + 4) = src[1];
-      if (n < N && mc < M) store_split8(turned + n * t_pitch + split_off(mc + (lane & 3) * 8), p);
+      if (n < N && mc < M) store_split8(turned + image_off(N, n, mc + (lane & 3) * 8), p);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -541,7 +544,6 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
   const int frow = lane & 15, fq = lane >> 4;
   if (producer) {
     constexpr int R = 2 * NI;                   // requests per wave and K-tile
-    const long pitch = pitch_of(w.K);
     unsigned voff_p[NI], voff_q[NI];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
@@ -549,20 +551,20 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
       const int kc = (lane & 7) ^ ((row >> 1) & 7);
       const int rp = w.m0 + row < w.M ? row : w.M - 1 - w.m0;
       const int rq = w.n0 + row < w.N ? row : w.N - 1 - w.n0;
-      voff_p[j] = (unsigned)rp * (unsigned)pitch + 16u * kc;
-      voff_q[j] = (unsigned)rq * (unsigned)pitch + 16u * kc;
+      voff_p[j] = 128 * rp + 16 * kc;
+      voff_q[j] = 128 * rq + 16 * kc;
     }
-    const __amdgpu_buffer_rsrc_t p_rsrc = rows_rsrc(w.P + w.m0 * pitch);
-    const __amdgpu_buffer_rsrc_t q_rsrc = rows_rsrc(w.Q + w.n0 * pitch);
     auto request = [&](int kt) {
       char* buf = smem + kt % NB * BUF_BYTES;
+      const __amdgpu_buffer_rsrc_t p_rsrc = tile_rsrc(w.P, w.M, w.m0, w.kt0 + kt);
+      const __amdgpu_buffer_rsrc_t q_rsrc = tile_rsrc(w.Q, w.N, w.n0, w.kt0 + kt);
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const int piece = wave * NI + j, at = (w.kt0 + kt) * 128;
+        const int piece = wave * NI + j;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(p_rsrc, (lds_void*)(buf + piece * 1024), 16,
-                                                 voff_p[j], at, 0, 0);
+                                                 voff_p[j], 0, 0, 0);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            q_rsrc, (lds_void*)(buf + OP_BYTES + piece * 1024), 16, voff_q[j], at, 0, 0);
+            q_rsrc, (lds_void*)(buf + OP_BYTES + piece * 1024), 16, voff_q[j], 0, 0, 0);
       }
     };
     for (int kt = 0; kt < NB - 1 && kt < w.nkt; ++kt) request(kt);
@@ -666,33 +668,30 @@ __device__ __forceinline__ void ns_wide_body(const NsArgs& args, int step, float
   const int wr = wave >> 1, wc = wave & 1;
   NsTile w;
   if (!ns_locate<BM, BN, TO>(args, step, w)) return;
-  const long pitch = pitch_of(w.K);
-
   // piece r of an operand: rows 8 (8 r + wave) .. + 7
   unsigned voff_p[RP], voff_q[RQ];
 #pragma unroll
   for (int r = 0; r < RP; ++r) {
     const int row = (r * 8 + wave) * 8 + (lane >> 3), kc = (lane & 7) ^ ((row >> 1) & 7);
-    voff_p[r] = (unsigned)(w.m0 + row < w.M ? row : w.M - 1 - w.m0) * (unsigned)pitch + 16u * kc;
+    voff_p[r] = 128 * (w.m0 + row < w.M ? row : w.M - 1 - w.m0) + 16 * kc;
   }
 #pragma unroll
   for (int r = 0; r < RQ; ++r) {
     const int row = (r * 8 + wave) * 8 + (lane >> 3), kc = (lane & 7) ^ ((row >> 1) & 7);
-    voff_q[r] = (unsigned)(w.n0 + row < w.N ? row : w.N - 1 - w.n0) * (unsigned)pitch + 16u * kc;
+    voff_q[r] = 128 * (w.n0 + row < w.N ? row : w.N - 1 - w.n0) + 16 * kc;
   }
-  const __amdgpu_buffer_rsrc_t p_rsrc = rows_rsrc(w.P + w.m0 * pitch);
-  const __amdgpu_buffer_rsrc_t q_rsrc = rows_rsrc(w.Q + w.n0 * pitch);
   // (behind the last K-tile the last one again, into a buffer nobody reads: the counts of the
   // waits stay the same)
   auto request = [&](int r, int kt, char* buf) {
-    const int at = (w.kt0 + (kt < w.nkt ? kt : w.nkt - 1)) * 128;
+    const int at = w.kt0 + (kt < w.nkt ? kt : w.nkt - 1);
     if (r < RP)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(p_rsrc, (lds_void*)(buf + (r * 8 + wave) * 1024), 16,
-                                               voff_p[r], at, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(tile_rsrc(w.P, w.M, w.m0, at),
+                                               (lds_void*)(buf + (r * 8 + wave) * 1024), 16,
+                                               voff_p[r], 0, 0, 0);
     else
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          q_rsrc, (lds_void*)(buf + P_BYTES + ((r - RP) * 8 + wave) * 1024), 16, voff_q[r - RP], at,
-          0, 0);
+          tile_rsrc(w.Q, w.N, w.n0, at),
+          (lds_void*)(buf + P_BYTES + ((r - RP) * 8 + wave) * 1024), 16, voff_q[r - RP], 0, 0, 0);
   };
   const int frow = lane & 15, fq = lane >> 4;
   const int p_hi = piece_off(wr * 64 + frow, fq), p_lo = piece_off(wr * 64 + frow, 4 + fq);
@@ -810,16 +809,15 @@ NsSizes sizes_of(long rows, long cols) {
   s.kn = up(s.n, 32);
   const long want = (rows * cols + 4095) / 4096;
   s.parts = want < NS_MAX_PARTS ? want : NS_MAX_PARTS;
-  s.x = up(s.m * pitch_of((int)s.kn), 256);
-  s.xt = up(s.n * pitch_of((int)s.km), 256);
-  s.sq = up(s.m * pitch_of((int)s.km), 256);
+  s.x = up(4 * s.m * s.kn, 256);
+  s.xt = up(4 * s.n * s.km, 256);
+  s.sq = up(4 * s.m * s.km, 256);
   s.a_parts = is_mid(rows, cols) ? mid_slabs(s.n) * MID_PART : 0;
   s.total = up(8 * s.parts, 256) + s.x + 2 * s.xt + 3 * s.sq + 2 * s.a_parts;
   return s;
 }
 
-// (a tile's rows lie within a 32-bit offset, 256 rows of 4 bytes an element; the tile counts of
-// 16 matrices within an int)
+// (the tile counts of 16 matrices lie within an int)
 bool bad_shape(long rows, long cols) {
   return rows < 1 || cols < 1 || rows > 4000000 || cols > 4000000 || rows * cols > (1L << 36);
 }

@@ -81,15 +81,16 @@ __device__ __forceinline__ void mid_put(char* to, int m, int n, f32x4 v) {
   *reinterpret_cast<uint2*>(to + mid_off(m, n, 1)) = lo;
 }
 
-// `rows` rows of an image, kts K-tiles each -> LDS; what is not there becomes zeros
-__device__ __forceinline__ void mid_request(const char* image, int rows, int kts, u32x4 (&v)[8]) {
+// rows r0 .. of an image of `rows` rows and kts K-tiles -> LDS; what is not there becomes zeros
+__device__ __forceinline__ void mid_request(const char* image, int rows, int r0, int kts,
+                                            u32x4 (&v)[8]) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const int piece = k * MID_THREADS + threadIdx.x;       // [4 K-tiles][128 rows][8]
     const int kt = piece >> 10, row = (piece >> 3) & 127, kc = piece & 7;
     v[k] = u32x4{0, 0, 0, 0};
-    if (row < rows && kt < kts)
-      v[k] = *reinterpret_cast<const u32x4*>(image + ((long)row * kts + kt) * 128 + kc * 16);
+    if (r0 + row < rows && kt < kts)
+      v[k] = *reinterpret_cast<const u32x4*>(image + image_off(rows, r0 + row, 32 * kt) + kc * 16);
   }
 }
 __device__ __forceinline__ void mid_land(char* to, const u32x4 (&v)[8]) {
@@ -118,7 +119,6 @@ __global__ __launch_bounds__(MID_THREADS) void ns_mid_kernel(MidArgs args, float
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, frow = lane & 15, fq = lane >> 4;
   const int wm = (wave >> 2) * 64, wn = (wave & 3) * 32;
   const bool tall = t.rows > t.cols;
-  const long xt_pitch = pitch_of(t.km);
   f32x4 acc[4][2];
   auto each = [&](auto&& f) {                    // f(i, j, row, first of four columns)
 #pragma unroll
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(MID_THREADS) void ns_mid_kernel(MidArgs args, float
     });
   } else {
     u32x4 held[8];
-    mid_request(t.xt0 + n0 * xt_pitch, width, t.km / 32, held);
+    mid_request(t.xt0, t.n, n0, t.km / 32, held);
     // A: the parts in slab order
     const __amdgpu_buffer_rsrc_t parts = __builtin_amdgcn_make_buffer_rsrc(
         (void*)t.a_parts[(args.turn + 1) & 1], 0, slabs * MID_PART, 0x00020000);
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(MID_THREADS) void ns_mid_kernel(MidArgs args, float
         *reinterpret_cast<u32x4*>(p) = src[0];
         *reinterpret_cast<u32x4*>(p + 4) = src[1];
         if (n < width && m < t.m)
-          store_split8(t.xt0 + (long)(n0 + n) * xt_pitch + split_off(m + (lane & 3) * 8), p);
+          store_split8(t.xt0 + image_off(t.n, n0 + n, m + (lane & 3) * 8), p);
       }
       __builtin_amdgcn_wave_barrier();
     }
