@@ -257,9 +257,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const char* image, i
 // Workgroups that share a K range of kt K-tiles when `most` are offered. Parts go through memory
 // and are waited for, 8 us a product at 1024 x 1024: a split is made where it takes 40 K-tiles or
 // more (0.2 us each on 64 x 64 tiles) out of a workgroup's way, in parts of 16 or more. Whole
-// call, split as here / never / as often as offered: 1024 x 1024 195 / 195 / 257 us, 2048 x 2048
-// 748 / 797 / 874, 300 x 8000 213 / 378 / 213, 1024 x 4096 371 / 403 / 398, 1024 x 8192 617 / 700 /
-// 850, 8192 x 4096 6.30 / 7.34 / 6.37 ms.
+// call, split as here / never / as often as offered: 1024 x 1024 183 / 182 / 247 us, 2048 x 2048
+// 714 / 766 / 716, 300 x 8000 175 / 275 / 174, 1024 x 4096 316 / 327 / 355, 1024 x 8192 421 / 458 /
+// 458, 8192 x 4096 5.33 / 7.52 / 5.31 ms.
 __host__ __device__ __forceinline__ int split_count(int kt, int most) {
   int s = kt / 16;
   s = s < most ? s : most;
@@ -302,7 +302,7 @@ __device__ __forceinline__ bool ns_locate(const NsArgs& args, int step, NsTile& 
     id = dtf_xcd_remap(blockIdx.x, args.unsplit);
   } else {
     // an XCD takes neighbouring tiles of one K range, whose rows its L2 holds (the parts of a tile
-    // side by side instead, so on several XCDs: 1024 x 8192 726 us, here 617)
+    // side by side instead, so on several XCDs: 1024 x 8192 in single steps 726 us, here 617)
     const int rest = args.first[args.count] - args.unsplit;
     w.splits = args.splits;
     const int r = dtf_xcd_remap(blockIdx.x - args.unsplit, rest * w.splits);
@@ -897,8 +897,8 @@ float product_us(const NsShape& shape, int tiles, int kt) {
 
 // The tile size that takes less time for a product; the wide one where they are close, because it
 // takes less power out of what the next product has. Measured (64 x 64 / 256 x 128, us): symmetric
-// products of 1024 x 1024 13 / 41, of 2048 x 2048 48 / 55, of 4096 x 4096 322 / 209; full ones of 1024 x
-// 1024 by 1024 x 4096 36 / 46, 2048 x 2048 by 2048 x 4096 142 / 95, 4096 x 4096 by 4096 x 8192 981 / 670.
+// products of 1024 x 1024 12 / 41, of 2048 x 2048 45 / 54, of 4096 x 4096 312 / 207; full ones of 1024 x
+// 1024 by 1024 x 4096 35 / 46, 2048 x 2048 by 2048 x 4096 133 / 98, 4096 x 4096 by 4096 x 8192 1013 / 668.
 int faster_tile(const int (&tiles)[2], int kt, float& us) {
   const float small = product_us(shape_of(64), tiles[0], kt);
   const float wide = product_us(shape_of(256), tiles[1], kt);
@@ -954,7 +954,7 @@ NsPlan plan_of(int count, const int* rows, const int* cols) {
 // Steps k and k + 1 taken as one. The second step's A is a polynomial of the first's, so X is
 // multiplied twice: A = X X^T, B = q(A), C = B A, A' = C B, B' = q'(A'), P = B' B, X = P X, where
 // single steps do it four times. For n = r m that is 3 r + 5 times m^3 instead of 6 r + 2 (2048 x
-// 8192 1.81 -> 1.40 ms, 8192 x 4096 6.46 -> 5.50, 1024 x 8192 0.60 -> 0.42). What is lost on A' acts on
+// 8192 1.71 -> 1.38 ms, 8192 x 4096 6.15 -> 5.33, 1024 x 8192 0.53 -> 0.42). What is lost on A' acts on
 // P only through B', beside a I: five steps of 4096 x 8192 are off by 2.0e-6 (single steps 2.3e-6, an
 // fp32 computation 5.6e-6), of 1024 x 4096 with a quarter of the rank by 8.1e-6 (6.6e-6, 9.0e-6).
 // Three steps as one would lose a^2 as much again. Odd counts have their single step before the

@@ -6,8 +6,8 @@
 // columns of X in place of one: every workgroup adds up A = X X^T from the slabs' parts, goes
 // through the polynomials of one step or of a pair of them by itself, multiplies its own slab, X =
 // P X, and leaves the slab's part of the next A. Five steps are five launches with the norm and the
-// first A: 128 x 128 63 us (tiled 89), 784 x 100 77 (109), 128 x 2048 93 (115), sixteen 128 x 2048 143
-// (166). A slab costs 0.7 us a launch to add up, so rows longer than 2048 are left to the tiles, and
+// first A: 128 x 128 64 us (tiled 86), 784 x 100 77 (105), 128 x 2048 93 (111), sixteen 128 x 2048 145
+// (163). A slab costs 0.7 us a launch to add up, so rows longer than 2048 are left to the tiles, and
 // so are calls with a larger matrix, whose launches take these along.
 //
 // What bounds it: 2 to 3 us a product on one CU, of which the matrix instructions are 1.3 and the
