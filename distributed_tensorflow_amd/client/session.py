@@ -82,6 +82,9 @@ def _graph_node_types(graph) -> Optional[List[int]]:
 _MUTATING_OPS = frozenset(("Assign", "AssignAdd", "AssignSub", "ApplyGradientDescent",
                            "MultiApplySGD", "ApplyOptimizer", "MultiApplyOptimizer",
                            "AffineUpdateVariable", "MultiMovingAverage"))
+# ops that update variables from gradients
+_UPDATE_OPS = frozenset(("ApplyGradientDescent", "MultiApplySGD", "ApplyOptimizer",
+                         "MultiApplyOptimizer"))
 _PACK_WORDS = 256     # fp32 words of pinned staging per captured step for small fetches
 
 
@@ -750,6 +753,7 @@ class Session:
                 if not any(n in redundant for n in order2):
                     rw, order = rw2, order2
 
+        order = self._gradients_first(order, rw, fed_set)
         plan = ExecutionPlan()
         slot_of: Dict[Tensor, int] = {}
 
@@ -821,6 +825,41 @@ class Session:
             self._plan_gradient_buckets(plan, {sl: t for t, sl in slot_of.items()})
         self._plan_gradient_views(plan)
         return plan
+
+    @staticmethod
+    def _gradients_first(order: List[Any], rw: fusion.Rewrite, fed_set: Set[Tensor]):
+        """The order of a plan with a Muon update: every gradient (and learning rate) of the
+        step's updates is computed before the first update writes a variable, whatever order the
+        updates run in -- the matrices' node and the vector optimizer's are two. What depends on
+        an update stays behind it."""
+        updates = [n for n in order if n.type in _UPDATE_OPS]
+        if not any(n.attrs.get("rule") == "muon" for n in updates):
+            return order
+
+        def resolve(node, t):
+            return t if t in fed_set or node.attrs.get("_raw_inputs") else rw.resolve(t)
+
+        def deps(node):
+            ins = [resolve(node, t) for _, t in value_inputs(node)]
+            return [t.op for t in ins if t not in fed_set] + \
+                [rw.resolve_op(c) for c in node.control_inputs]
+
+        behind: Set[Any] = set()               # updates, and what depends on one
+        for n in order:
+            if n.type in _UPDATE_OPS or any(d in behind for d in deps(n)):
+                behind.add(n)
+        ahead: Set[Any] = set()                # what the updates' gradients are computed from
+        stack = [t.op for u in updates for t in (resolve(u, t) for _, t in value_inputs(u))
+                 if t not in fed_set]
+        while stack:
+            n = stack.pop()
+            if n not in ahead:
+                ahead.add(n)
+                stack.extend(deps(n))
+        first = order.index(updates[0])
+        moved = [n for n in order[first:] if n in ahead and n not in behind]
+        kept = set(moved)
+        return order[:first] + moved + [n for n in order[first:] if n not in kept]
 
     def _plan_gradient_views(self, plan: ExecutionPlan) -> None:
         """Under a multi-rank collective runtime the gradients the optimizer step consumes are
