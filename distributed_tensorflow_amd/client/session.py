@@ -82,9 +82,11 @@ def _graph_node_types(graph) -> Optional[List[int]]:
 _MUTATING_OPS = frozenset(("Assign", "AssignAdd", "AssignSub", "ApplyGradientDescent",
                            "MultiApplySGD", "ApplyOptimizer", "MultiApplyOptimizer",
                            "AffineUpdateVariable", "MultiMovingAverage"))
-# ops that update variables from gradients
+# ops that update variables from gradients, and the ops whose output may be their input's storage
 _UPDATE_OPS = frozenset(("ApplyGradientDescent", "MultiApplySGD", "ApplyOptimizer",
                          "MultiApplyOptimizer"))
+_VIEW_OPS = frozenset(("Identity", "StopGradient", "Reshape", "ReshapeLike", "Cast", "Transpose",
+                       "SumToShapeOf", "BroadcastLike", "ReduceGrad", "AddN"))
 _PACK_WORDS = 256     # fp32 words of pinned staging per captured step for small fetches
 
 
@@ -753,7 +755,7 @@ class Session:
                 if not any(n in redundant for n in order2):
                     rw, order = rw2, order2
 
-        order = self._gradients_first(order, rw, fed_set)
+        order, copies = self._gradients_first(order, rw, fed_set)
         plan = ExecutionPlan()
         slot_of: Dict[Tensor, int] = {}
 
@@ -784,7 +786,7 @@ class Session:
             raw = node.attrs.get("_raw_inputs")
             for i, t in value_inputs(node):
                 rt = t if (t in fed_set or raw) else rw.resolve(t)
-                ins[i] = slot(rt)
+                ins[i] = slot(copies.get((node, i), rt))
             outs = [slot(o) for o in node.outputs]
             step = _Step(node, kernel, ins, outs, d.host_only)
             if d.host_only:
@@ -828,13 +830,14 @@ class Session:
 
     @staticmethod
     def _gradients_first(order: List[Any], rw: fusion.Rewrite, fed_set: Set[Tensor]):
-        """The order of a plan with a Muon update: every gradient (and learning rate) of the
-        step's updates is computed before the first update writes a variable, whatever order the
-        updates run in -- the matrices' node and the vector optimizer's are two. What depends on
-        an update stays behind it."""
+        """``(order, copies)`` of a plan with a Muon update: every gradient (and learning rate) of
+        the step's updates is computed before the first update writes a variable, whatever order
+        the updates run in -- the matrices' node and the vector optimizer's are two. A gradient
+        that is a variable's own storage, of a variable that the step updates, is read from a copy
+        made there: ``copies[update node, input]``. What depends on an update stays behind it."""
         updates = [n for n in order if n.type in _UPDATE_OPS]
         if not any(n.attrs.get("rule") == "muon" for n in updates):
-            return order
+            return order, {}
 
         def resolve(node, t):
             return t if t in fed_set or node.attrs.get("_raw_inputs") else rw.resolve(t)
@@ -859,7 +862,37 @@ class Session:
         first = order.index(updates[0])
         moved = [n for n in order[first:] if n in ahead and n not in behind]
         kept = set(moved)
-        return order[:first] + moved + [n for n in order[first:] if n not in kept]
+        written: Set[Any] = set()
+        for u in updates:
+            if "var_ops" in u.attrs:
+                written.update(u.attrs["var_ops"])
+                written.update(s for slots in u.attrs.get("slot_ops", ()) for s in slots)
+            else:
+                written.update(t.op for t in u.inputs[:u.attrs.get("num_refs", 1)])
+        copies, snapshots, made = {}, [], {}
+        for u in updates:
+            for i, t in value_inputs(u):
+                t = source = resolve(u, t)
+                if t in fed_set or t.op in behind:
+                    continue
+                while source not in fed_set and source.op.type in _VIEW_OPS:
+                    source = resolve(source.op, source.op.inputs[0])
+                if source in fed_set:
+                    continue
+                var = source.op if source.op.type in _VAR_TYPES else \
+                    source.op.inputs[0].op if source.op.type in _MUTATING_OPS and \
+                    source.op.inputs else None
+                if var not in written:
+                    continue
+                if t not in made:
+                    node = fusion.FusedNode(u.graph, "Snapshot", t.op.name + "/snapshot", [t],
+                                            [(t.dtype, t.shape)], {"_raw_inputs": True},
+                                            device=t.op.device)
+                    snapshots.append(node)
+                    made[t] = node.outputs[0]
+                copies[u, i] = made[t]
+        return order[:first] + moved + snapshots + \
+            [n for n in order[first:] if n not in kept], copies
 
     def _plan_gradient_views(self, plan: ExecutionPlan) -> None:
         """Under a multi-rank collective runtime the gradients the optimizer step consumes are

@@ -208,6 +208,19 @@ def _cast(op, inputs, ctx):
     return _fallback("Cast", op, inputs, ctx)
 
 
+@hip_kernel("Snapshot")
+def _snapshot(op, inputs, ctx):
+    x = inputs[0]
+    if not x.is_cuda:                  # read from another process: host memory
+        return [x.clone()]
+    if not x.is_contiguous():
+        return _fallback("Snapshot", op, inputs, ctx)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.numel():
+        hip.copy_2d(x.view(1, -1), out.view(1, -1))
+    return [out]
+
+
 @hip_kernel("RowScale")
 def _row_scale(op, inputs, ctx):
     x, s = inputs

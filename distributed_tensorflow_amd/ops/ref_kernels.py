@@ -431,6 +431,12 @@ ref_kernel("Identity")(_un(lambda x: x))
 ref_kernel("StopGradient")(_un(lambda x: x))
 
 
+@ref_kernel("Snapshot")
+def _snapshot(op, inputs, ctx):
+    """The value as it is now, in memory of its own (updates read what they overwrite from it)."""
+    return [inputs[0].clone()]
+
+
 @ref_kernel("Cast")
 def _cast(op, inputs, ctx):
     return [inputs[0].to(op.attrs["dtype"].torch)]

@@ -1,4 +1,4 @@
-"""Updates whose gradients go through variables that the same step writes: every gradient is the
+"""Updates whose gradients are read from variables that the same step writes: every gradient is the
 value before the step, however many updates the step has, fused or one by one, on either device.
 
 Tolerance: the orthogonalised update is off by at most 2e-3 in the spectral norm (see
@@ -31,6 +31,83 @@ def _rule(w, grads, lr=0.05, mu=0.95):
         v = mu * v + g
         w = w - lr * max(1.0, w.shape[1] / w.shape[0]) ** 0.5 * _ns64(g + mu * v)
     return w
+
+
+def _step(device, fusion, values, pairs):
+    """One step of ``pairs(variables)`` -> [(gradient, variable)]; the variables afterwards."""
+    with tf.Graph().as_default():
+        ws = [tf.Variable(tf.constant(v), name="w%d" % i) for i, v in enumerate(values)]
+        train = tf.train.MuonOptimizer(0.05).apply_gradients(pairs(ws))
+        with tf.Session(config=tf.ConfigProto(device=device, graph_fusion=fusion)) as sess:
+            sess.run(tf.global_variables_initializer())
+            sess.run(train)
+            got = sess.run(ws)
+            assert sess.stats["torch_fallbacks"] == 0 or device == "cpu"
+            return got
+
+
+def _near(got, want, updates):
+    s = max(1.0, want.shape[1] / want.shape[0]) ** 0.5
+    assert np.abs(got - want).max() <= updates * 0.05 * s * 2e-3
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fusion", [True, False])
+@pytest.mark.parametrize("read", ["loss", "identity", "itself", "turned"])
+def test_a_variable_updated_twice(device, fusion, read):
+    rng = np.random.RandomState(5)
+    values = [rng.randn(*s).astype(np.float32) for s in ((70, 90), (12, 10), (33, 33))]
+
+    def pairs(ws):
+        if read == "loss":
+            g = [tf.gradients(tf.nn.l2_loss(w), [w._variable])[0] for w in ws]
+        elif read == "identity":
+            g = [tf.identity(w) for w in ws]
+        elif read == "itself":
+            g = [w._variable for w in ws]
+        else:
+            g = [tf.reshape(tf.identity(w), [w.shape[0], w.shape[1]]) for w in ws]
+        return [*zip(g, ws), *zip([tf.identity(x) for x in g], ws)]
+    for w, got in zip(values, _step(device, fusion, values, pairs)):
+        _near(got, _rule(w, [w, w]), 2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fusion", [True, False])
+@pytest.mark.parametrize("computed", [False, True])
+def test_variables_that_are_each_other_s_gradients(device, fusion, computed):
+    rng = np.random.RandomState(6)
+    values = [rng.randn(*s).astype(np.float32) for s in ((66, 70), (66, 70), (66, 70))]
+
+    def pairs(ws):
+        g = [tf.identity(ws[(i + 1) % 3]) for i in range(3)]
+        if computed:
+            g = [tf.multiply(x, 2.0) for x in g]
+        return list(zip(g, ws))
+    out = _step(device, fusion, values, pairs)
+    for i, w in enumerate(values):
+        _near(out[i], _rule(w, [values[(i + 1) % 3]]), 1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fusion", [True, False])
+def test_a_momentum_as_gradient(device, fusion):
+    """The second step's gradient is the momentum that the update advances."""
+    rng = np.random.RandomState(7)
+    w0, g0 = (rng.randn(40, 72).astype(np.float32) for _ in range(2))
+    with tf.Graph().as_default():
+        w = tf.Variable(tf.constant(w0), name="w")
+        opt = tf.train.MuonOptimizer(0.05)
+        first = opt.apply_gradients([(tf.constant(g0), w)])
+        m = opt.get_slot(w, "momentum")
+        second = opt.apply_gradients([(tf.identity(m), w)])
+        with tf.Session(config=tf.ConfigProto(device=device, graph_fusion=fusion)) as sess:
+            sess.run(tf.global_variables_initializer())
+            sess.run(first)
+            sess.run(second)
+            got, gm = sess.run([w, m])
+    _near(got, _rule(w0, [g0, g0]), 2)
+    np.testing.assert_allclose(gm, 1.95 * g0, rtol=1e-6)
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -70,3 +147,19 @@ def test_vectors_and_matrices_of_one_step(device, fusion, vectors, order):
             np.testing.assert_allclose(got, v - 0.5 * g, rtol=1e-4, atol=1e-4)
         else:
             assert np.abs(got - _rule(v, [g], lr=5.0)).max() <= 5.0 * 2e-3
+
+
+@pytest.mark.parametrize("fusion", [True, False])
+def test_a_read_behind_an_assignment_is_the_new_value(fusion):
+    """A gradient that is read behind another write of the step is that write's value."""
+    rng = np.random.RandomState(8)
+    w0, w1 = (rng.randn(20, 30).astype(np.float32) for _ in range(2))
+    with tf.Graph().as_default():
+        w = tf.Variable(tf.constant(w0), name="w")
+        with tf.control_dependencies([w.assign(tf.constant(w1))]):
+            g = tf.identity(w)
+        train = tf.train.MuonOptimizer(0.05).apply_gradients([(g, w), (tf.identity(g), w)])
+        with tf.Session(config=tf.ConfigProto(device="cpu", graph_fusion=fusion)) as sess:
+            sess.run(tf.global_variables_initializer())
+            sess.run(train)
+            _near(sess.run(w), _rule(w1, [w1, w1]), 2)
