@@ -7,15 +7,21 @@
 //
 // Arithmetic. The three products of a step are bound by the matrix cores, and fp32 operands run
 // there at a sixteenth of the 16-bit rate. So every operand is held as a pair of fp16 numbers,
-// hi = fp16(x) and lo = fp16(x - hi): together 22 bits of x, at most 2^-23 of it lost (fp32 itself
-// loses 2^-24). A product is hi hi + hi lo + lo hi with fp32 accumulation; lo lo (2^-22 of the
-// term) is left out. Polynomial steps grow a small singular value by up to `a` each and carry the
-// rounding noise of the operands along, 485-fold over five default steps: single 16-bit operands
-// are off by 1e-2 of the result's size on matrices of bounded rank, this form by less than an
-// fp32 computation is (its accumulators take 32 or 64 terms at a time). fp16 and not bf16
+// hi = fp16(x) and lo = fp16(2^11 (x - hi)): together 22 bits of x, at most 2^-23 of it lost (fp32
+// itself loses 2^-24). A product is hi hi + 2^-11 (hi lo + lo hi) with fp32 accumulation, the two
+// parts in accumulators of their own; lo lo (2^-22 of the term) is left out. fp16 and not bf16
 // because 11 + 11 bits in three products do what bf16 needs six for; its range is met by powers
 // of two: entries of X are at most 3.5 in size (host-checked for the coefficients), stored times
-// 2^14; A and B times 2^12.
+// 2^14; A and B times 2^12. The factor 2^11 of lo keeps both halves normal numbers for entries of
+// X down to 2^-28 and of A and B down to 2^-26; below, an entry is off by at most 2^-50 and 2^-48.
+// So a row that is eight decades smaller than the others keeps its own digits, as it does in
+// fp32: 4096 x 8192 with rows spread over eight decades, the worst row is off by 5e-5 of itself
+// (fp32 4e-5; 1e-1 with lo = x - hi unscaled, for 0.5 % of the time).
+//
+// Polynomial steps grow a small singular value by up to `a` each and carry the rounding noise of
+// the operands along, 485-fold over five default steps: single 16-bit operands are off by 1e-2 of
+// the result's size on matrices of bounded rank, this form by less than an fp32 computation is
+// (its sums hold 128 elements before they are emptied).
 //
 // Work. A and B are symmetric: only tiles on and below the diagonal are computed, each written
 // to both places. a I is part of B, so X is not read again for the sum. B X needs the columns of
@@ -42,6 +48,7 @@ constexpr int NS_MAX_STEPS = 32;
 constexpr int NS_SLOTS = 512;          // workgroups of a product that run at once, at most
 constexpr int NS_MAX_PARTS = 1024;     // workgroups that share a matrix's sum of squares
 constexpr float X_SCALE = 16384.f, AB_SCALE = 4096.f;
+constexpr float LO_SCALE = 2048.f;     // of the small halves
 constexpr double X_LIMIT = 3.5, AB_LIMIT = 15.0;   // times the scales: below fp16's 65504
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -104,7 +111,7 @@ __device__ __forceinline__ int matrix_of(const NsArgs& args, int id) {
 // hi | lo << 16
 __device__ __forceinline__ unsigned split_pack(float v) {
   const _Float16 hi = (_Float16)v;
-  const _Float16 lo = (_Float16)(v - (float)hi);
+  const _Float16 lo = (_Float16)((v - (float)hi) * LO_SCALE);
   return (unsigned)__builtin_bit_cast(unsigned short, hi) |
          (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
 }
@@ -113,11 +120,15 @@ __device__ __forceinline__ unsigned split_pack(float v) {
 __device__ __forceinline__ void split4(f32x4 v, uint2& hi, uint2& lo) {
   const f16x2 h0 = __builtin_convertvector(f32x2{v[0], v[1]}, f16x2);
   const f16x2 h1 = __builtin_convertvector(f32x2{v[2], v[3]}, f16x2);
-  const f32x2 r0 = {v[0] - (float)h0[0], v[1] - (float)h0[1]};
-  const f32x2 r1 = {v[2] - (float)h1[0], v[3] - (float)h1[1]};
+  const f32x2 r0 = {(v[0] - (float)h0[0]) * LO_SCALE, (v[1] - (float)h0[1]) * LO_SCALE};
+  const f32x2 r1 = {(v[2] - (float)h1[0]) * LO_SCALE, (v[3] - (float)h1[1]) * LO_SCALE};
   hi = uint2{__builtin_bit_cast(unsigned, h0), __builtin_bit_cast(unsigned, h1)};
   lo = uint2{__builtin_bit_cast(unsigned, __builtin_convertvector(r0, f16x2)),
              __builtin_bit_cast(unsigned, __builtin_convertvector(r1, f16x2))};
+}
+
+__device__ __forceinline__ float joined(_Float16 hi, _Float16 lo) {
+  return __builtin_fmaf((float)lo, 1.f / LO_SCALE, (float)hi);
 }
 
 // eight packed elements -> 16 bytes of hi, 16 bytes of lo
@@ -291,6 +302,17 @@ struct NsTile {
   int kt0, nkt;              // this workgroup's K-tiles
   int mat, shared, split, splits;
 };
+
+template <int NM, int NN>
+__device__ __forceinline__ void add_cross(f32x4 (&sum)[NM][NN], const f32x4 (&cross)[NM][NN]) {
+#pragma unroll
+  for (int i = 0; i < NM; ++i)
+#pragma unroll
+    for (int j = 0; j < NN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        sum[i][j][r] = __builtin_fmaf(cross[i][j][r], 1.f / LO_SCALE, sum[i][j][r]);
+}
 
 // this workgroup's tile; false: nothing to do
 template <int BM, int BN, int TO>
@@ -476,7 +498,7 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArg
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             v[r] = __builtin_fmaf(cc / AB_SCALE, v[r],
-                                  __builtin_fmaf(cb, (float)ah[r] + (float)al[r],
+                                  __builtin_fmaf(cb, joined(ah[r], al[r]),
                                                  m == n + r ? ca * AB_SCALE : 0.f));
         }
 #pragma unroll
@@ -583,7 +605,11 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
     asm volatile("s_barrier" ::: "memory");
     if (w.splits == 1) return;
   } else {
-    f32x4 acc[NI][NI];
+    f32x4 acc[NI][NI], cross[NI][NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) cross[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     // fragments of two K-tiles: one is read while the other is multiplied
     f16x8 ph[2][NI], pl[2][NI], qh[2][NI], ql[2][NI];
     auto fetch = [&](int kt, auto odd) {
@@ -618,9 +644,9 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
         for (int j = 0; j < NI; ++j) {
           // (operands swapped: a lane's four results lie along N)
           const f32x4 from = FIRST ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j];
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[S][j], ph[S][i], from, 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[S][j], pl[S][i], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[S][j], ph[S][i], acc[i][j], 0, 0, 0);
+          cross[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[S][j], ph[S][i], cross[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[S][j], ph[S][i], from, 0, 0, 0);
+          cross[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[S][j], pl[S][i], cross[i][j], 0, 0, 0);
         }
     };
     asm volatile("s_barrier" ::: "memory");       // K-tile 0 has landed
@@ -638,6 +664,7 @@ __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, floa
 #pragma unroll
         for (int j = 0; j < NI; ++j) sum[i][j] += acc[i][j];
     }
+    add_cross(sum, cross);
     // the buffers become the epilogue's scratch
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
@@ -700,11 +727,11 @@ __device__ __forceinline__ void ns_wide_body(const NsArgs& args, int step, float
   auto fragment = [&](const char* at, int i) {   // (16 rows further: the same swizzle)
     return *reinterpret_cast<const f16x8*>(at + i * 2048);
   };
-  f32x4 sum[NI][NI], acc[NI][NI];
+  f32x4 sum[NI][NI], acc[NI][NI], cross[NI][NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NI; ++j) sum[i][j] = cross[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -732,9 +759,10 @@ __device__ __forceinline__ void ns_wide_body(const NsArgs& args, int step, float
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         // (operands swapped: a lane's four results lie along N)
-        const f32x4 from = FIRST && term == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j];
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            term == 0 ? ql[j] : qh[j], term == 1 ? pl[i] : ph[i], from, 0, 0, 0);
+        f32x4& to = term == 2 ? acc[i][j] : cross[i][j];
+        const f32x4 from = FIRST && term == 2 ? f32x4{0.f, 0.f, 0.f, 0.f} : to;
+        to = __builtin_amdgcn_mfma_f32_16x16x32_f16(term == 0 ? ql[j] : qh[j],
+                                                    term == 1 ? pl[i] : ph[i], from, 0, 0, 0);
       }
       if (term == 0 && i + 1 < NI) {
         ph[i + 1] = fragment(buf + p_hi, i + 1);
@@ -755,6 +783,7 @@ __device__ __forceinline__ void ns_wide_body(const NsArgs& args, int step, float
 #pragma unroll
       for (int j = 0; j < NI; ++j) sum[i][j] += acc[i][j];
   }
+  add_cross(sum, cross);
   // the buffers become the epilogue's scratch
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   if (w.splits > 1 && !ns_join<NI, NI, 512>(sum, args, w)) return;

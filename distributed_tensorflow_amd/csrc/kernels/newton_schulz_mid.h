@@ -38,10 +38,11 @@ template <int KT>
 __device__ __forceinline__ void mid_product(const char* P, const char* Q, int m0, int n0,
                                             f32x4 (&acc)[4][2]) {
   const int lane = threadIdx.x & 63, frow = lane & 15, fq = lane >> 4;
+  f32x4 cross[4][2];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 2; ++j) acc[i][j] = cross[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
     f16x8 ph[4], pl[4], qh[2], ql[2];
@@ -62,11 +63,12 @@ __device__ __forceinline__ void mid_product(const char* P, const char* Q, int m0
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         // (operands swapped: a lane's four results lie along the columns)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph[i], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl[i], acc[i][j], 0, 0, 0);
+        cross[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[j], ph[i], cross[i][j], 0, 0, 0);
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], ph[i], acc[i][j], 0, 0, 0);
+        cross[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[j], pl[i], cross[i][j], 0, 0, 0);
       }
   }
+  add_cross(acc, cross);
 }
 
 // byte offset of elements n .. n + 3 of row m (hi; n a multiple of four) in a matrix of pairs
@@ -203,7 +205,7 @@ __global__ __launch_bounds__(MID_THREADS) void ns_mid_kernel(MidArgs args, float
         for (int r = 0; r < 4; ++r)
           acc[i][j][r] = __builtin_fmaf(
               c[2] / AB_SCALE, acc[i][j][r],
-              __builtin_fmaf(c[1], (float)hi[r] + (float)lo[r],
+              __builtin_fmaf(c[1], joined(hi[r], lo[r]),
                              m == n + r && m < t.m ? c[0] * AB_SCALE : 0.f));
       });
     };

@@ -1338,7 +1338,8 @@ def newton_schulz(g, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
     X = a X + (b A + c A A) X`` on the orientation with fewer rows. Every singular value is moved
     towards one and the singular vectors are kept. ``coefficients``: one (a, b, c), or one per
     step; a polynomial under which a singular value in [0, 1] grows beyond 3.5 is refused. The
-    products keep 22 bits of every operand and accumulate in fp32; the result is rounded once, to
+    products keep 22 bits of every operand down to 2^-26 and accumulate in fp32, so rows and columns
+    up to eight decades smaller than others keep their own digits; the result is rounded once, to
     ``g``'s dtype. Up to 16 matrices share one sequence of launches."""
     what = "newton_schulz"
     if isinstance(g, torch.Tensor):

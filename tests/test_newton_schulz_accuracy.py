@@ -8,6 +8,14 @@ the sums, which hold at most 128 elements before they are emptied. So the kernel
 the fp32 form's relative error on the same input, and 16 steps of 2^-24 where that is tiny. A
 product that is left without its small halves is off by 2^-11 of itself: a thousand times as much.
 
+Rows (or columns) of very different size are compared row by row: a small row passes through the
+products beside large ones and must keep its own digits. What is smaller than fp16's normal numbers
+is absolute: an entry of X is off by at most 2^-50 and one of A or B by 2^-48 (X has norm one at the
+start). The first is 2^-50 sqrt(n) on a row of n elements, taken again in every step while the row
+grows 3.4-fold: 1.4 times that in all. The second meets rows of X of norm about one, m of them with
+errors of random sign: 2^-48 sqrt(m). Both, relative to the row of X: ``floor``, under 2^-48
+(sqrt(m) + sqrt(n)) over the smallest row's norm (300 x 1000, six decades: 7e-7; eight: 6e-5).
+
 The thin form (up to 64 rows or columns) computes in 64 bits and rounds once: half a step of the
 result, plus what the steps make of the 64-bit sums' rounding. A sum of 64 products of size one is
 off by 10 * 2^-53. An error of the first A, between a direction that is nearly empty and one that is
@@ -41,6 +49,12 @@ def whole(x, want):
     return (torch.linalg.norm(x.double() - want) / torch.linalg.norm(want)).item()
 
 
+def by_lines(x, want, dim):
+    """The worst row's (dim 1) or column's (dim 0) error, relative to itself."""
+    off, size = (torch.linalg.norm(t, dim=dim) for t in (x.double() - want, want))
+    return (off / size).max().item()
+
+
 def bound(fp32_error):
     return 2.0 * fp32_error + 16 * 2.0 ** -24
 
@@ -65,19 +79,27 @@ def matrix(rows, cols, kind, seed=0, device="cpu"):
     return g.to(device)
 
 
+def floor(g, dim):
+    x = g.double()
+    x = x / torch.linalg.norm(x)
+    smallest = torch.linalg.norm(x, dim=dim).min().item()
+    return 2.0 ** -48 * (min(g.shape) ** 0.5 + g.shape[dim] ** 0.5) / smallest
+
+
 # ---------------------------------------------------------------------------------------
 # without a GPU: the scheme in torch, and what it is without one of its parts
 # ---------------------------------------------------------------------------------------
-X_SCALE, AB_SCALE = 2.0 ** 14, 2.0 ** 12
+X_SCALE, AB_SCALE, LO_SCALE = 2.0 ** 14, 2.0 ** 12, 2.0 ** 11
 
 
-def scheme(g, steps=5, cross=(True, True), last=(True, True)):
+def scheme(g, steps=5, lo_scale=LO_SCALE, cross=(True, True), last=(True, True)):
     """The kernels' arithmetic with exact sums, rounded to fp32 behind every product. ``cross``:
-    which of hi lo and lo hi are added (``last``: in the last product)."""
+    which of hi lo and lo hi are added (``last``: in the last product); ``lo_scale``: of the small
+    halves."""
     def image(x, scale):
         s = x.double() * scale
         hi = s.to(torch.float16).double()
-        return hi, (s - hi).to(torch.float16).double()
+        return hi, ((s - hi) * lo_scale).to(torch.float16).double() / lo_scale
 
     def product(p, q, scale, terms=cross):
         r = p[0] @ q[0].t()
@@ -108,6 +130,15 @@ def test_the_bound_notices_a_missing_half(kind):
     for broken in (dict(cross=(True, False)), dict(cross=(False, True)), dict(last=(False, True)),
                    dict(last=(False, False)), dict(cross=(False, False))):
         assert whole(scheme(g, **broken), want) > 4 * limit, broken
+
+
+@pytest.mark.parametrize("decades", [6, 8])
+def test_the_bound_notices_small_halves_without_their_scale(decades):
+    g = matrix(130, 300, "rows%d" % decades)
+    want = formula(g, torch.float64)
+    limit = bound(by_lines(formula(g, F32), want, 1)) + floor(g, 1)
+    assert by_lines(scheme(g), want, 1) <= limit
+    assert by_lines(scheme(g, lo_scale=1.0), want, 1) > 2 * limit
 
 
 def test_the_thin_bound_notices_fp32():
@@ -145,6 +176,19 @@ def test_errors_beside_plain_fp32(hip, form, kind):
         want = formula(g, torch.float64)
         limit = bound(whole(formula(g, F32), want))
         assert whole(got, want) <= limit, (tuple(g.shape), whole(got, want), limit)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["rows4", "rows6", "rows8", "cols6", "cols8"])
+@pytest.mark.parametrize("form", sorted(FORMS))
+def test_rows_and_columns_of_different_size(hip, form, kind):
+    """Each keeps its own digits, as it does in fp32."""
+    mats = [matrix(r, c, kind, i, "cuda") for i, (r, c) in enumerate(FORMS[form])]
+    dim = 1 if kind.startswith("rows") else 0
+    for g, got in zip(mats, hip.newton_schulz(mats)):
+        want = formula(g, torch.float64)
+        limit = bound(by_lines(formula(g, F32), want, dim)) + floor(g, dim)
+        assert by_lines(got, want, dim) <= limit, (tuple(g.shape), by_lines(got, want, dim), limit)
 
 
 @pytest.mark.gpu
