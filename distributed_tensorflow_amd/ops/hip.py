@@ -1298,6 +1298,7 @@ def multi_optim(rule: str, params: Sequence[torch.Tensor], grads: Sequence[torch
 
 NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _NS_GROUP = 16          # matrices of one launch sequence
+_NS_MAX_DIM, _NS_MAX_SIZE = 4000000, 1 << 36
 
 
 def _ns_coefficients(coefficients, steps: int, what: str):
@@ -1311,17 +1312,28 @@ def _ns_coefficients(coefficients, steps: int, what: str):
     return (ctypes.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
 
 
-def _ns_workspace(shapes, device, what: str):
-    n = len(shapes)
-    rows = (ctypes.c_int * n)(*[s[0] for s in shapes])
-    cols = (ctypes.c_int * n)(*[s[1] for s in shapes])
-    size = lib().dtf_newton_schulz_workspace(n, rows, cols)
-    if size <= 0:
-        raise HipKernelError("%s: matrices of up to 4000000 rows and columns, got %s"
-                             % (what, list(shapes)))
+def _ns_groups(shapes, device, what: str):
+    """[(start, end, rows, cols)] of the launch sequences for matrices of ``shapes``, and a workspace
+    that fits each of them (they run one after the other): (tensor, aligned address, bytes). All
+    that can be refused is refused here, before the first launch."""
+    for r, c in shapes:
+        if r > _NS_MAX_DIM or c > _NS_MAX_DIM or r * c > _NS_MAX_SIZE:
+            raise HipKernelError("%s: matrices of up to %d rows and columns and 2^36 elements, got %s"
+                                 % (what, _NS_MAX_DIM, (r, c)))
+    groups, size = [], 0
+    for start in range(0, len(shapes), _NS_GROUP):
+        part = shapes[start:start + _NS_GROUP]
+        n = len(part)
+        rows = (ctypes.c_int * n)(*[s[0] for s in part])
+        cols = (ctypes.c_int * n)(*[s[1] for s in part])
+        need = lib().dtf_newton_schulz_workspace(n, rows, cols)
+        if need <= 0:
+            raise HipKernelError("%s: unsupported shapes %s" % (what, list(part)))
+        size = max(size, need)
+        groups.append((start, start + n, rows, cols))
     ws = torch.empty((size,), dtype=torch.uint8, device=device)
     base = (ws.data_ptr() + 255) // 256 * 256
-    return rows, cols, ws, base, ws.data_ptr() + size - base
+    return groups, (ws, base, ws.data_ptr() + size - base)
 
 
 def _ns_check(code: int, what: str) -> None:
@@ -1366,15 +1378,17 @@ def newton_schulz(g, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
         result = outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in mats]
     work = [(t if t.is_contiguous() else t.contiguous(), o) for t, o in zip(mats, outs)
             if t.numel()]
-    for start in range(0, len(work), _NS_GROUP):
-        part = work[start:start + _NS_GROUP]
-        n, t0 = len(part), part[0][0]
-        rows, cols, ws, base, size = _ns_workspace([t.shape for t, _ in part], t0.device, what)
+    if not work:
+        return result
+    device = mats[0].device
+    groups, (ws, base, size) = _ns_groups([t.shape for t, _ in work], device, what)
+    for start, end, rows, cols in groups:
+        n, part = end - start, work[start:end]
         g_arr = (ctypes.c_void_p * n)(*[t.data_ptr() for t, _ in part])
         o_arr = (ctypes.c_void_p * n)(*[o.data_ptr() for _, o in part])
-        _ns_check(_launch_on(t0.device, lib().dtf_newton_schulz, (
-            n, g_arr, o_arr, rows, cols, _NORM_TYPES[t0.dtype], steps, coef, float(epsilon), base,
-            size)), what)
+        _ns_check(_launch_on(device, lib().dtf_newton_schulz, (
+            n, g_arr, o_arr, rows, cols, _NORM_TYPES[mats[0].dtype], steps, coef, float(epsilon),
+            base, size)), what)
     return result
 
 
@@ -1392,7 +1406,8 @@ def multi_muon(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     ``u = g + momentum v`` (``nesterov``; else ``v``); ``w = (1 - lr weight_decay) w - lr scale
     newton_schulz(u)``. ``scales``: one factor per parameter, default ``sqrt(max(1, outputs /
     inputs))`` of its [inputs, outputs]. ``lr``: a number, or an fp32 device scalar read when the
-    kernels run. Up to 16 matrices of any shapes share one sequence of launches."""
+    kernels run. Up to 16 matrices of any shapes share one sequence of launches. A call that is
+    refused has updated nothing."""
     what = "multi_muon"
     if len(params) != len(grads) or len(params) != len(moments) or \
             (scales is not None and len(scales) != len(params)):
@@ -1433,15 +1448,15 @@ def multi_muon(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
             for a, b, c in (zip(p, g, m) if p.dim() == 3 else ((p, g, m),))]
     if lr_dev is not None and work and lr_dev.device != work[0][0].device:
         raise HipKernelError("multi_muon: lr is on another device")
-    c = ctypes
-    for start in range(0, len(work), _NS_GROUP):
-        part = work[start:start + _NS_GROUP]
-        n, w0 = len(part), part[0][0]
-        rows, cols, ws, base, size = _ns_workspace([w.shape for w, _, _, _ in part], w0.device,
-                                                   what)
+    if not work:
+        return
+    c, device = ctypes, work[0][0].device
+    groups, (ws, base, size) = _ns_groups([w.shape for w, _, _, _ in work], device, what)
+    for start, end, rows, cols in groups:
+        n, part = end - start, work[start:end]
         arrays = [(c.c_void_p * n)(*[t[k].data_ptr() for t in part]) for k in range(3)]
         s_arr = (c.c_float * n)(*[t[3] for t in part])
-        _ns_check(_launch_on(w0.device, lib().dtf_multi_muon_f32, (
+        _ns_check(_launch_on(device, lib().dtf_multi_muon_f32, (
             n, arrays[0], arrays[1], arrays[2], s_arr, rows, cols, steps, coef, float(epsilon),
             float(lr), _ptr(lr_dev), float(momentum), int(bool(nesterov)), float(weight_decay),
             base, size)), what)

@@ -794,7 +794,7 @@ def _optim_launch(ctx, rule, hyper, var_ops, slot_ops_list, power_ops, grads, lr
     """Update every variable whose storage, slots and powers are local fp32 GPU tensors with the
     multi-tensor kernel; returns the (var_op, slot_ops, grad) triples it could not take."""
     powers = [_local_f32(ctx, p) for p in power_ops]
-    rest, ps, gs, s0, s1 = [], [], [], [], []
+    rest, ps, gs, s0, s1, stores = [], [], [], [], [], []
     if lr is not None and not (_is_f32(lr) and lr.is_cuda and lr.numel() == 1):
         return list(zip(var_ops, slot_ops_list, grads))
     for var_op, slot_ops, g in zip(var_ops, slot_ops_list, grads):
@@ -810,7 +810,7 @@ def _optim_launch(ctx, rule, hyper, var_ops, slot_ops_list, power_ops, grads, lr
             s0.append(slots[0])
         if len(slots) > 1:
             s1.append(slots[1])
-        ctx.session._store_for(var_op).update_count += 1
+        stores.append(ctx.session._store_for(var_op))
     if ps and rule == "muon":
         from .ref_kernels import muon_rule
         h, coef, _ = muon_rule(hyper, ps[0].shape)
@@ -828,6 +828,8 @@ def _optim_launch(ctx, rule, hyper, var_ops, slot_ops_list, power_ops, grads, lr
                            coef, h["epsilon"])
     elif ps:
         hip.multi_optim(rule, ps, gs, s0, s1, hyper, powers, lr=lr)
+    for store in stores:               # (a refused call has updated nothing)
+        store.update_count += 1
     return rest
 
 
