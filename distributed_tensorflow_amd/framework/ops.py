@@ -709,31 +709,67 @@ def clip_by_value(t, clip_value_min, clip_value_max, name=None) -> Tensor:
 NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
-def newton_schulz(t, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
-                  epsilon: float = 1e-7, name=None) -> Tensor:
-    """``t`` -- a matrix, or a stack of matrices of rank 3 -- with its singular values moved
-    towards one by ``steps`` Newton-Schulz products (``X = t / (|t| + epsilon)``, then ``X = a X +
-    (b A + c A A) X`` with ``A = X X^T``): an update of equal size in every direction, between
-    ``compute_gradients`` and ``apply_gradients`` like ``clip_by_norm``. ``coefficients``: one
-    (a, b, c) or one per step. Not differentiable."""
-    t = convert_to_tensor(t)
-    if t.dtype.name not in ("float32", "bfloat16", "float16"):
-        raise TypeError("newton_schulz: fp32, bf16 or fp16 input, got %s" % t.dtype.name)
-    if t.shape is None or len(t.shape) not in (2, 3):
-        raise ValueError("newton_schulz needs a matrix or a stack of matrices, got shape %s"
-                         % (t.shape,))
-    steps = int(steps)
+def newton_schulz_steps(steps: int, coefficients):
+    """((a, b, c) of every step) from one triple or one per step. The GPU kernels hold X and the
+    polynomials as 16-bit pairs, so a singular value in [0, 1] may grow to 3.5 and a polynomial to
+    15 at most; other coefficients are refused on every device, when the graph is built."""
     if not 1 <= steps <= 32:
         raise ValueError("newton_schulz: steps must be 1..32, got %d" % steps)
     rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else coefficients
     if len(rows) != steps or any(len(r) != 3 for r in rows):
         raise ValueError("newton_schulz: coefficients are one (a, b, c) or one for each of the %d "
                          "steps" % steps)
+    rows = tuple(tuple(float(v) for v in r) for r in rows)
+    top = 1.0 + 1e-6                                  # the largest singular value
+    for row in rows:
+        # p(s) = s q(s^2), q(t) = a + b t + c t^2, t in [0, top^2]: the extremes of p and q lie
+        # at the ends and where q' or p' is zero
+        a, b, c = (float(np.float32(v)) for v in row)
+        with np.errstate(all="ignore"):
+            root = np.sqrt(np.maximum(9.0 * b * b - 20.0 * a * c, 0.0))
+            t = np.array([0.0, top * top] + [np.divide(u, v) for u, v in (
+                (-b, 2.0 * c), (-3.0 * b + root, 10.0 * c), (-3.0 * b - root, 10.0 * c),
+                (-a, 3.0 * b))])
+            t = t[(t >= 0.0) & (t <= top * top)]
+            q = np.abs(a + b * t + c * t * t)
+            p = (np.sqrt(t) * q).max()
+        if not (np.abs([a, b, c]).sum() < 1e30 and top * top <= 15.0 and q.max() <= 15.0
+                and p <= 3.5):
+            raise ValueError("newton_schulz: coefficients %r let a singular value in [0, 1] grow "
+                             "beyond 3.5 (or their polynomial beyond 15)" % (row,))
+        top = p * (1.0 + 1e-3)                        # (rounding of what is computed)
+    return rows
+
+
+def newton_schulz_shape(shape) -> None:
+    """Refuses matrices (the last two dimensions) that the kernels do not take."""
+    r, c = (1 if d is None else int(d) for d in tuple(shape)[-2:])
+    if max(r, c) > 4000000 or r * c > 1 << 36:
+        raise ValueError("newton_schulz: matrices of up to 4000000 rows and columns and 2^36 "
+                         "elements, got %s" % (tuple(shape),))
+
+
+def newton_schulz(t, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
+                  epsilon: float = 1e-7, name=None) -> Tensor:
+    """``t`` -- a matrix, or a stack of matrices of rank 3 -- with its singular values moved
+    towards one by ``steps`` Newton-Schulz products (``X = t / (|t| + epsilon)``, then ``X = a X +
+    (b A + c A A) X`` with ``A = X X^T``): an update of equal size in every direction, between
+    ``compute_gradients`` and ``apply_gradients`` like ``clip_by_norm``. ``coefficients``: one
+    (a, b, c) or one per step; those under which a singular value in [0, 1] grows beyond 3.5 are
+    refused. Not differentiable."""
+    t = convert_to_tensor(t)
+    if t.dtype.name not in ("float32", "bfloat16", "float16"):
+        raise TypeError("newton_schulz: fp32, bf16 or fp16 input, got %s" % t.dtype.name)
+    if t.shape is None or len(t.shape) not in (2, 3):
+        raise ValueError("newton_schulz needs a matrix or a stack of matrices, got shape %s"
+                         % (t.shape,))
+    newton_schulz_shape(t.shape)
+    steps = int(steps)
+    rows = newton_schulz_steps(steps, coefficients)
     if not epsilon >= 0.0:
         raise ValueError("newton_schulz: epsilon must not be negative, got %r" % (epsilon,))
     return _op1("NewtonSchulz", [t], t.dtype, t.shape, name=name or "newton_schulz", steps=steps,
-                coefficients=tuple(tuple(float(v) for v in r) for r in rows),
-                epsilon=float(epsilon))
+                coefficients=rows, epsilon=float(epsilon))
 
 
 # ---------------------------------------------------------------------------------------

@@ -313,18 +313,13 @@ class MuonOptimizer(Optimizer):
         super().__init__(use_locking, name)
         self._learning_rate, self._lr_tensor = self._split_lr(learning_rate)
         steps = int(steps)
-        if not 1 <= steps <= 32:
-            raise ValueError("steps must be 1..32, got %d" % steps)
-        rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else coefficients
-        if len(rows) != steps or any(len(r) != 3 for r in rows):
-            raise ValueError("coefficients are one (a, b, c) or one for each of the %d steps"
-                             % steps)
+        rows = F.newton_schulz_steps(steps, coefficients)
         if not epsilon >= 0.0 or rms_scale < 0.0:
             raise ValueError("epsilon and rms_scale must not be negative")
         # (the order of ref_kernels.MUON_HYPER)
         self._hyper = (self._learning_rate, float(momentum), float(bool(use_nesterov)),
                        float(weight_decay), float(rms_scale), float(epsilon), float(steps),
-                       *[float(v) for r in rows for v in r])
+                       *[v for r in rows for v in r])
         self._vector_optimizer = vector_optimizer
 
     @staticmethod
@@ -338,6 +333,7 @@ class MuonOptimizer(Optimizer):
                              "%s" % ", ".join(v.op.name for v in vectors))
         for v in var_list:
             if self._is_matrix(v):
+                F.newton_schulz_shape(v.shape)
                 self._zeros_slot(v, "momentum", self._name, per_element=False)
         self._has_vectors = bool(vectors)
         if vectors:

@@ -25,6 +25,53 @@ def test_shapes_beyond_the_kernels_range_are_refused_on_the_host():
     assert size >= hip.lib().dtf_newton_schulz_workspace(2, ints(96, 96), ints(80, 80)) - 256
 
 
+@pytest.mark.parametrize("rows", [(9.0, 0.0, 0.0), (float("nan"), 0.0, 0.0), (20.0, -40.0, 20.0),
+                                  (1.0, float("inf"), 0.0), [COEF, (4.0, 0.0, 0.0)]])
+def test_coefficients_are_refused_where_the_graph_is_built(rows):
+    steps = 2 if hasattr(rows[0], "__len__") else 5
+    with pytest.raises(ValueError, match="grow beyond"):
+        tf.newton_schulz(tf.placeholder(tf.float32, [6, 4]), steps=steps, coefficients=rows)
+    with pytest.raises(ValueError, match="grow beyond"):
+        tf.train.MuonOptimizer(0.1, steps=steps, coefficients=rows)
+
+
+def test_matrices_beyond_the_kernels_range_are_refused_where_the_graph_is_built():
+    for shape in ([4000001, 3], [2, 3, 4000001], [300000, 300000], [None, 4000001]):
+        with pytest.raises(ValueError, match="matrices of up to"):
+            tf.newton_schulz(tf.placeholder(tf.float32, shape))
+    tf.newton_schulz(tf.placeholder(tf.float32, [None, 40]))
+    w = tf.Variable(tf.zeros([4000001, 1]), name="long")
+    with pytest.raises(ValueError, match="matrices of up to"):
+        tf.train.MuonOptimizer(0.1).apply_gradients([(tf.identity(w), w)])
+
+
+def test_graph_and_library_refuse_the_same_coefficients():
+    from distributed_tensorflow_amd.framework.ops import newton_schulz_steps
+    from distributed_tensorflow_amd.ops import hip
+    if not hip.library_present():
+        pytest.skip("native library not built")
+    rng = np.random.RandomState(0)
+    lib, ints, ptrs = hip.lib(), ctypes.c_int * 1, ctypes.c_void_p * 1
+    taken = 0
+    for trial in range(400):
+        steps = int(rng.randint(1, 6))
+        rows = [tuple(np.array(COEF) * (1 + 0.3 * rng.randn(3)) * rng.choice([1.0, 0.0, 1.0, 1.0], 3))
+                for _ in range(steps)]
+        if trial % 10 == 0:
+            rows = [(1.5, -0.5, 0.0)] * steps
+        # (no workspace: -1 once the coefficients are taken, -2 before)
+        code = lib.dtf_newton_schulz(1, ptrs(4096), ptrs(4096), ints(96), ints(80), 0, steps,
+                                     (ctypes.c_float * (3 * steps))(*[v for r in rows for v in r]),
+                                     1e-7, 4096, 0, None)
+        try:
+            newton_schulz_steps(steps, rows)
+            assert code == -1, rows
+            taken += 1
+        except ValueError:
+            assert code == -2, rows
+    assert 60 < taken < 340
+
+
 @pytest.fixture(scope="module")
 def hip():
     assert torch.cuda.is_available(), "gpu tests need a GPU"
