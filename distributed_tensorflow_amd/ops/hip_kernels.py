@@ -709,7 +709,8 @@ def _assign_add_kernel(sign: float, type_name: str):
         if p is not None and _is_f32(delta) and delta.is_cuda \
                 and (delta.shape == p.shape or delta.numel() == 1):
             return [hip.assign_add(p, delta, sign)]
-        if p is None and not getattr(ctx.session._store_for(var_op), "local_tensor", None):
+        fast = getattr(ctx.session._store_for(var_op), "local_tensor", None)
+        if fast is None or fast(var_op.name) is None:
             # the variable lives in another process (parameter server): the store ships it
             return [ctx.var_assign_add(var_op, delta if sign > 0 else -delta)]
         return _fallback(type_name, op, inputs, ctx)
