@@ -287,12 +287,16 @@ class ExecContext:
     def note_fallback(self, op, why: str = "") -> None:
         """A GPU kernel wrapper has no native code for this case (see ``ops/hip_kernels``)."""
         sess = self.session
-        entry = (op.type, op.name, why)
         if self.device.type == "cuda" and not sess.config.allow_torch_fallback:
             from ..ops.hip import HipKernelError
             raise HipKernelError(
                 "op %s (%s) has no gfx950 kernel for %s; refusing to run torch kernels on the GPU "
                 "(ConfigProto(allow_torch_fallback=True) permits it)" % (op.name, op.type, why))
+        self.count_fallback(op, why)
+
+    def count_fallback(self, op, why: str = "") -> None:
+        sess = self.session
+        entry = (op.type, op.name, why)
         sess.stats["torch_fallbacks"] += 1
         if len(sess.fallback_log) < 256 and entry not in sess.fallback_log:
             sess.fallback_log.append(entry)

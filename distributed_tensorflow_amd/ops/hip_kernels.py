@@ -791,6 +791,46 @@ def _multi_apply_sgd(op, inputs, ctx):
     return []
 
 
+def _muon_launch(hyper, ps, gs, vs, lr) -> None:
+    """The "muon" rule on fp32 GPU matrices, in place."""
+    from .ref_kernels import muon_rule
+    h, coef, _ = muon_rule(hyper, ps[0].shape)
+    hip.multi_muon(ps, [g.view(p.shape) for p, g in zip(ps, gs)], vs,
+                   h["lr"] if lr is None else lr, h["momentum"], bool(h["nesterov"]),
+                   h["weight_decay"], [muon_rule(hyper, p.shape)[2] for p in ps], int(h["steps"]),
+                   coef, h["epsilon"])
+
+
+def _muon_through_stores(op, ctx, rest, lr):
+    """(new values, what is left) of "muon" updates whose variables or momenta live elsewhere (a
+    parameter server): the rule runs in one call on copies of the values this step has read, and
+    the differences are shipped as ``apply_rule_through_stores`` ships them. What is left (matrices
+    that are not fp32) goes through torch there and is counted as such."""
+    todo, left = [], []
+    for item in rest:
+        var_op, slot_ops, g = item
+        w, v = ctx.var_read(var_op), ctx.var_read(slot_ops[0])
+        if all(_is_f32(t) and t.is_cuda and t.is_contiguous() for t in (w, v, g)) \
+                and (lr is None or (_is_f32(lr) and lr.is_cuda)):
+            todo.append((item, w, v, hip.axpby(1.0, w), hip.axpby(1.0, v)))
+        else:
+            if w.is_cuda:
+                ctx.count_fallback(op, "muon of %s" % ", ".join(str(t.dtype) for t in (w, v, g)))
+            left.append(item)
+    if todo:
+        _muon_launch(op.attrs["hyper"], [t[3] for t in todo], [t[0][2] for t in todo],
+                     [t[4] for t in todo], lr)
+    out = []
+    for (var_op, slot_ops, _), w, v, new_w, new_v in todo:
+        store = ctx.session._store_for(slot_ops[0])
+        if getattr(store, "local_tensor", lambda n: None)(slot_ops[0].name) is not None:
+            ctx.var_assign(slot_ops[0], new_v)
+        else:
+            ctx.var_assign_add(slot_ops[0], hip.axpby(1.0, new_v, -1.0, v))
+        out.append(ctx.var_apply_sgd(var_op, 1.0, hip.axpby(1.0, w, -1.0, new_w)))
+    return out, left
+
+
 def _optim_launch(ctx, rule, hyper, var_ops, slot_ops_list, power_ops, grads, lr=None) -> list:
     """Update every variable whose storage, slots and powers are local fp32 GPU tensors with the
     multi-tensor kernel; returns the (var_op, slot_ops, grad) triples it could not take."""
@@ -813,8 +853,6 @@ def _optim_launch(ctx, rule, hyper, var_ops, slot_ops_list, power_ops, grads, lr
             s1.append(slots[1])
         stores.append(ctx.session._store_for(var_op))
     if ps and rule == "muon":
-        from .ref_kernels import muon_rule
-        h, coef, _ = muon_rule(hyper, ps[0].shape)
         left = list(zip(ps, gs, s0))
         while left:                        # (a variable that is updated twice: one after the other)
             first = {}
@@ -822,11 +860,7 @@ def _optim_launch(ctx, rule, hyper, var_ops, slot_ops_list, power_ops, grads, lr
                 first.setdefault(item[0].data_ptr(), item)
             left = [item for item in left if first[item[0].data_ptr()] is not item]
             now = list(first.values())
-            hip.multi_muon([p for p, _, _ in now], [g.view(p.shape) for p, g, _ in now],
-                           [v for _, _, v in now], h["lr"] if lr is None else lr, h["momentum"],
-                           bool(h["nesterov"]), h["weight_decay"],
-                           [muon_rule(hyper, p.shape)[2] for p, _, _ in now], int(h["steps"]),
-                           coef, h["epsilon"])
+            _muon_launch(hyper, *([t[k] for t in now] for k in range(3)), lr)
     elif ps:
         hip.multi_optim(rule, ps, gs, s0, s1, hyper, powers, lr=lr)
     for store in stores:               # (a refused call has updated nothing)
@@ -867,6 +901,10 @@ def _apply_optimizer(op, inputs, ctx):
     grad = ctx.reduce_gradients([inputs[-1]], [var_op])[0]
     rest = _optim_launch(ctx, op.attrs["rule"], op.attrs["hyper"], [var_op], [slot_ops],
                          power_ops, [grad], lr)
+    if op.attrs["rule"] == "muon" and rest:
+        done, rest = _muon_through_stores(op, ctx, rest, lr)
+        if done:
+            return done
     for v, s_ops, g in rest:       # state in another process (parameter server)
         return [apply_rule_through_stores(ctx, op.attrs["rule"], op.attrs["hyper"], v, s_ops,
                                           power_ops, g, lr)]
@@ -898,6 +936,8 @@ def _multi_apply_optimizer(op, inputs, ctx):
         grads = ctx.reduce_gradients(grads, var_ops)   # no-op without a sync runtime
     rest = _optim_launch(ctx, op.attrs["rule"], op.attrs["hyper"], var_ops, slot_ops,
                          op.attrs["power_ops"], grads, lr)
+    if op.attrs["rule"] == "muon" and rest:
+        _, rest = _muon_through_stores(op, ctx, rest, lr)
     for v, s_ops, g in rest:
         apply_rule_through_stores(ctx, op.attrs["rule"], op.attrs["hyper"], v, s_ops,
                                   op.attrs["power_ops"], g, lr)
