@@ -13,7 +13,10 @@
 //
 // Everything between a load and a store is fp32. The variance is that of the differences from
 // the first mean, and what those differences sum to corrects both (the "corrected two-pass"
-// form): a row far from zero loses nothing but the rounding of its mean.
+// form): a row far from zero loses nothing but the rounding of its mean. The first mean of a
+// constant row is off by the rounding of its sum, D 2^-24 of the value for sums D additions deep
+// (up to 40 where the row lies in registers); the correction takes that out but for D 2^-24 of
+// itself. So y is beta up to D^2 2^-48 |x| / sqrt(eps): 2e-6 for 1000 and the default epsilon.
 #include "elem.h"
 
 namespace {
@@ -131,7 +134,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layer_norm_kernel(
       for (int k = 0; k < V; ++k) s += v[j][k];
     }
     group_sum2<L>(s, q, my_red, lane, turn);
-    const float m0 = s / (float)cols;     // (a constant row is its mean exactly)
+    const float m0 = s / (float)cols;
     s = q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -190,7 +193,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(
       for (int k = 0; k < V; ++k) s += v[k];
     }
     group_sum2<L>(s, q, red, lane, turn);
-    const float m0 = s / (float)cols;     // (a constant row is its mean exactly)
+    const float m0 = s / (float)cols;
     s = q = 0.f;
     for (long c = lane * V; c < cols; c += L * V) {
       load_part<V>(xr, (int)c, cols, v);
