@@ -200,8 +200,8 @@ def optimizer_rule_step(rule: str, hyper, w, g, s0, s1=None, powers=None):
         h, coef, scale = muon_rule(hyper, tuple(w.shape))
         s0 = h["momentum"] * s0 + g
         u = g + h["momentum"] * s0 if h["nesterov"] else s0
-        o = torch.stack([newton_schulz(m, coef, h["epsilon"]) for m in u]) if u.dim() == 3 \
-            else newton_schulz(u, coef, h["epsilon"])
+        o = newton_schulz(u, coef, h["epsilon"]) if u.dim() == 2 else u if not len(u) else \
+            torch.stack([newton_schulz(m, coef, h["epsilon"]) for m in u])
         w = (1.0 - h["lr"] * h["weight_decay"]) * w - (h["lr"] * scale) * o
     else:
         raise ValueError("unknown optimizer rule %r" % (rule,))

@@ -45,6 +45,21 @@ def test_matrices_beyond_the_kernels_range_are_refused_where_the_graph_is_built(
         tf.train.MuonOptimizer(0.1).apply_gradients([(tf.identity(w), w)])
 
 
+@pytest.mark.parametrize("shape", [(0, 4, 5), (3, 0, 5), (0, 4), (4, 0)])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+def test_empty_variables_are_updated_to_themselves(shape, device):
+    with tf.Graph().as_default():
+        w = tf.Variable(tf.zeros(list(shape)), name="none")
+        full = tf.Variable(tf.ones([2, 3]), name="some")
+        train = tf.train.MuonOptimizer(0.1).apply_gradients(
+            [(tf.zeros(list(shape)), w), (tf.ones([2, 3]), full)])
+        with tf.Session(config=tf.ConfigProto(device=device)) as sess:
+            sess.run(tf.global_variables_initializer())
+            sess.run(train)
+            a, b = sess.run([w, full])
+    assert a.shape == shape and np.abs(b - 1.0).max() > 0
+
+
 def test_graph_and_library_refuse_the_same_coefficients():
     from distributed_tensorflow_amd.framework.ops import newton_schulz_steps
     from distributed_tensorflow_amd.ops import hip
