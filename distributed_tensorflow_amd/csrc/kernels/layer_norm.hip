@@ -173,7 +173,9 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layer_norm_kernel(
   }
 }
 
-// rows longer than the registers of 1024 lanes: the same sums with the row read three times
+// rows longer than the registers of 1024 lanes: the same sums with the row read three times, the
+// later ones in part from the L2 (bf16 4096 x 20000: 107 us, where one read and one write take 64;
+// 1024 x 65536: 80 and 52; fp32 172 and 104)
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void layer_norm_long_kernel(
     const T* __restrict__ x, long ldx, const P* __restrict__ gamma, const P* __restrict__ beta,
@@ -365,7 +367,9 @@ __global__ __launch_bounds__(grad_block(L)) void layer_norm_grad_kernel(
   }
 }
 
-// long rows: dx with two reads of the row, one workgroup per row ...
+// long rows: dx with two reads of the row, one workgroup per row ... (with the column sums, which
+// read x and dy once more, an element per lane: bf16 4096 x 20000 243 us, where the bytes take 95;
+// 1024 x 65536: 200 and 78; fp32 359 and 156)
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(
     const T* __restrict__ dy, long ldd, const T* __restrict__ x, long ldx,

@@ -16,7 +16,7 @@
 // X down to 2^-28 and of A and B down to 2^-26; below, an entry is off by at most 2^-50 and 2^-48.
 // So a row that is eight decades smaller than the others keeps its own digits, as it does in
 // fp32: 4096 x 8192 with rows spread over eight decades, the worst row is off by 5e-5 of itself
-// (fp32 4e-5; 1e-1 with lo = x - hi unscaled, for 0.5 % of the time).
+// (fp32 4e-5; with lo = x - hi unscaled 1e-1). The factor costs up to 1 % of the time.
 //
 // Polynomial steps grow a small singular value by up to `a` each and carry the rounding noise of
 // the operands along, 485-fold over five default steps: single 16-bit operands are off by 1e-2 of
@@ -288,9 +288,10 @@ __device__ __forceinline__ int piece_off(int row, int kc) {
 // type.
 //
 // Accumulation. The matrix instruction adds its 32 products to the accumulator in steps of its
-// own; a long chain of them loses more than fp32 sums of rounded products do (1024 x 1024: the
-// result was off by 4.7e-6, an fp32 computation by 3.1e-6). Every NS_CHAIN K-tiles the
-// accumulators are added to a second set and start again from zero (2.2e-6; no time).
+// own; a long chain of them loses what the pairs gain (a gradient of 1024 x 1024: the result was off
+// by 3.0e-6, an fp32 computation by 3.1e-6). Every NS_CHAIN K-tiles the accumulators of hi hi are
+// added to a second set and start again from zero (1.8e-6; no time). The products with the small
+// halves count 2^-11 of themselves and stay in one chain.
 //
 // Splits. A tile whose K range is shared leaves fp32 partial tiles in memory; the workgroup that
 // arrives last adds all of them in split order, whoever it is, so the bits do not depend on the
@@ -543,9 +544,12 @@ __device__ __forceinline__ void ns_store(const f32x4 (&acc)[NM][NN], const NsArg
 // 64 x 64 tiles: four multiplying waves and four that issue the LDS-DMA requests, three K-tiles
 // ahead into four buffers -- the multiplying waves never wait at the address unit. Two workgroups
 // per CU. (Four waves that do both: 1024 x 1024 302 us instead of 186.) A workgroup that has its CU to
-// itself takes 0.23 us per K-tile, the time the 16 KB of requests take: six and eight buffers, or
-// requests to registers and stores from there, were 10 to 20 % slower. Two on a CU are bound by
-// the LDS: 48 KB in and out per K-tile.
+// itself takes 0.23 us per K-tile: every 16 KB has a wait and a barrier of its own, and their
+// latency is what bounds it. (LDS-DMA alone brings 16 KB in 0.07 us, with a barrier per 64 KB in
+// 0.12, profiles/lds_fill_rate_probe.jsonl; the matrix units are busy for 7 to 14 %.) Six and eight
+// buffers, or requests to registers and stores from there, were 10 to 20 % slower. Two on a CU take
+// 0.51 us for a K-tile each, 96 KB through the LDS at 78 bytes per clock of the 263 that the probe's
+// mix of requests and reads reaches, the matrix units busy for 18 to 27 %: the same waits.
 template <typename E, int TO, bool MUON>
 __device__ __forceinline__ void ns_small_body(const NsArgs& args, int step, float ca, float cb,
                                               float cc, const NsMuon& mo) {
@@ -984,8 +988,8 @@ NsPlan plan_of(int count, const int* rows, const int* cols) {
 // multiplied twice: A = X X^T, B = q(A), C = B A, A' = C B, B' = q'(A'), P = B' B, X = P X, where
 // single steps do it four times. For n = r m that is 3 r + 5 times m^3 instead of 6 r + 2 (2048 x
 // 8192 1.71 -> 1.38 ms, 8192 x 4096 6.15 -> 5.33, 1024 x 8192 0.53 -> 0.42). What is lost on A' acts on
-// P only through B', beside a I: five steps of 4096 x 8192 are off by 2.0e-6 (single steps 2.3e-6, an
-// fp32 computation 5.6e-6), of 1024 x 4096 with a quarter of the rank by 8.1e-6 (6.6e-6, 9.0e-6).
+// P only through B', beside a I: five steps of 4096 x 8192 are off by 1.7e-6 (single steps 2.1e-6, an
+// fp32 computation 5.6e-6), of 1024 x 4096 with a quarter of the rank by 6.5e-6 (5.5e-6, 9.0e-6).
 // Three steps as one would lose a^2 as much again. Odd counts have their single step before the
 // last pair, where the singular values are least apart. P has to fit the images of B.
 bool step_pairs(int k, int steps, const double* factor) {

@@ -1352,7 +1352,8 @@ def newton_schulz(g, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS,
     step; a polynomial under which a singular value in [0, 1] grows beyond 3.5 is refused. The
     products keep 22 bits of every operand down to 2^-26 and accumulate in fp32, so rows and columns
     up to eight decades smaller than others keep their own digits; the result is rounded once, to
-    ``g``'s dtype. Up to 16 matrices share one sequence of launches."""
+    ``g``'s dtype. Up to 16 matrices share one sequence of launches. The same call gives the same
+    bits; a matrix of more than 64 rows and columns may be rounded otherwise beside larger ones."""
     what = "newton_schulz"
     if isinstance(g, torch.Tensor):
         mats = [g] if g.dim() == 2 else list(g) if g.dim() == 3 else None
