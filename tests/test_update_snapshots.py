@@ -163,3 +163,38 @@ def test_a_read_behind_an_assignment_is_the_new_value(fusion):
             sess.run(tf.global_variables_initializer())
             sess.run(train)
             _near(sess.run(w), _rule(w1, [w1, w1]), 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fusion", [True, False])
+def test_captured_steps_copy_what_they_overwrite(fusion):
+    """Replays read the variables as each step finds them: the same bits as eager steps."""
+    rng = np.random.RandomState(10)
+    values = [rng.randn(*s).astype(np.float32) for s in ((70, 90), (70, 90), (24, 10))]
+    bx = rng.randn(8, 24).astype(np.float32)
+    runs = []
+    for graphs in (True, False):
+        with tf.Graph().as_default():
+            ws = [tf.Variable(tf.constant(v), name="w%d" % i) for i, v in enumerate(values)]
+            b = tf.Variable(tf.zeros([10]), name="b")
+            x = tf.placeholder(tf.float32, [8, 24])
+            loss = tf.reduce_sum(tf.square(tf.add(tf.matmul(x, ws[2]), b)))
+            g2, gb = tf.gradients(loss, [ws[2]._variable, b._variable])
+            opt = tf.train.MuonOptimizer(0.05, vector_optimizer=tf.train.MomentumOptimizer(0.01, 0.9))
+            train = opt.apply_gradients([(tf.identity(ws[1]), ws[0]), (tf.identity(ws[0]), ws[1]),
+                                         (g2, ws[2]), (gb, b), (tf.identity(ws[0]), ws[0])])
+            with tf.Session(config=tf.ConfigProto(device="cuda:0", graph_fusion=fusion,
+                                                  hip_graphs=graphs)) as sess:
+                sess.run(tf.global_variables_initializer())
+                got = []
+                for _ in range(6):
+                    sess.run([train, loss], {x: bx})
+                    got.append(sess.run(ws + [b]))
+                runs.append((got, dict(sess.stats)))
+    assert runs[0][1]["graph_replays"] >= 2 and runs[1][1]["graph_replays"] == 0
+    assert runs[0][1]["torch_fallbacks"] == 0
+    for a, b in zip(runs[0][0], runs[1][0]):
+        for u, v in zip(a, b):
+            assert np.array_equal(u, v)
+    _near(runs[0][0][0][0], _rule(values[0], [values[1], values[0]]), 2)
+    _near(runs[0][0][0][1], _rule(values[1], [values[0]]), 1)
